@@ -75,6 +75,11 @@ extern "C" {
 /* combine: order in which a token's rows are added */
 #define OMNI_ORDER_SLOT 0 /* ascending sorted slot  (npu_grouped_matmul_finalize_routing) */
 #define OMNI_ORDER_K 1    /* ascending k            (npu_moe_finalize_routing) */
+/* sandwich norm: what the gate is indexed by */
+#define OMNI_GATE_NONE 0
+#define OMNI_GATE_CHANNEL 1 /* [H] */
+#define OMNI_GATE_TOKEN 2   /* [rows], row stride ld_gate */
+#define OMNI_GATE_FULL 3    /* [rows, H], row stride ld_gate */
 
 /* Last error message of the calling thread ("" if none). */
 const char* omni_moe_last_error(void);
@@ -145,6 +150,58 @@ int omni_dynamic_quant(const void* x, int in_dtype, int64_t rows, int cols, int6
 int omni_add_rms_norm_quant(const void* x_bf16, const void* residual_bf16, const void* weight_bf16, int64_t rows,
                             int H, float eps, void* residual_out_bf16, void* y_bf16, int8_t* q, float* scale,
                             void* stream);
+
+/*
+ * The norm after a block, the block's gate and residual scale, the residual sum and the norm before the next block
+ * (+ per-token dynamic quantisation of its result) in one pass, for models with a norm on both sides of a block; the
+ * same place in a layer as RMSNorm.forward with a residual (omni/models/common/layers/layernorm.py:13-32).
+ * x, residual, post_weight [H], pre_weight [H], gate, residual_out, y: one dtype of OMNI_DT_*; x, residual, gate and
+ * residual_out have row strides (elements), y and q are rows x H without gaps; H <= 16384, any alignment of an element.
+ *   t  = x / sqrt(mean(x*x) + post_eps) * post_weight;  r' = residual + (residual_scale * gate) * t;
+ *   y  = r' / sqrt(mean(r'*r') + pre_eps) * pre_weight  (r' before its rounding; fp32 throughout, one rounding per output)
+ *   scale = max|y| / 127, q = rint(y / scale) on the rounded y; a zero row gives 0, 0; a row with an infinity or a NaN
+ *   gives zeros and that infinity or NaN as its scale.
+ * y, q (with scale) may be NULL.  residual_out may be residual itself (same stride) and y may be x without gaps; no
+ * other output may overlap an input.  At most 2^22 - 1 rows.
+ */
+int omni_sandwich_norm(const void* x, int dtype, int64_t ldx, const void* residual, int64_t ld_residual,
+                       const void* post_weight, const void* pre_weight, const void* gate, int gate_mode, int64_t ld_gate,
+                       int64_t rows, int H, float post_eps, float pre_eps, float residual_scale, void* residual_out,
+                       int64_t ld_residual_out, void* y, int8_t* q, float* scale, void* stream);
+
+/*
+ * SwiGLU of rows in memory (npu_swiglu, omni/models/common/layers/activation.py:29) and, with q and scale, the
+ * npu_dynamic_quant that follows it in front of a quantised projection.
+ *   gate_up [rows, 2I] of dtype with row stride ld (elements): gate channels first;
+ *   h = silu(gate) * up rounded once to dtype;  scale = max|h| / 127, q = rint(h / scale) on the rounded h (zero rows and
+ *   rows that are not finite as for omni_sandwich_norm).
+ * h or q (with scale) may be NULL.  I <= 32768, any alignment of an element, at most 2^22 - 1 rows; no output may
+ * overlap the input.
+ */
+int omni_swiglu_quant(const void* gate_up, int dtype, int64_t ld, int64_t rows, int I, void* h, int8_t* q, float* scale,
+                      void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection (the quantised weights of the projection cannot take
+ * an adapter in; ReplicatedLinear / MergedReplicatedLinear, omni/models/common/layers/linear.py:620-762, are where it
+ * is added here).
+ *   out[t, :] = base[t, :] + (scale[g] * (x[t, :] . A[g]^T)) . B[g]^T for the adapter g of token t, base[t, :] without one
+ * x [T,H], base and out [T,N] bf16 or fp16 with row strides; A [n, n_slices*r, H], B [n, N, r], scale [n] fp32 or NULL
+ * (1).  N is the sum of `widths` (HOST array of n_slices, at most 4): the columns of slice j are multiplied with columns
+ * [j*r, (j+1)*r) of x . A^T.  Both products are summed in fp32, the first one is carried with 16 (bf16) or 22 (fp16)
+ * bits of mantissa into the second; out is rounded once.  The result of a token does not depend on other tokens' values;
+ * its last bits may depend on T and n, which choose how the first sum is cut.
+ *   sorted_src, offsets: of omni_moe_permute(ids, T, K = 1, lo = 0, hi = n, OMNI_IDX_TOKEN_MAJOR).  Ids outside [0, n):
+ *   no adapter.
+ *   H, r, every width, ldx, ld_base, ld_out multiples of 8, pointers 16-byte aligned; r <= 256, n <= 256, H and N <= 2^20.
+ *   out may be base (same stride): rows without an adapter are then left alone.  No other overlap.
+ *   workspace: omni_adapter_linear_workspace_bytes(T, n, H, r, n_slices), 16-byte aligned; written and read by this call.
+ */
+int omni_adapter_linear(const void* x, int dtype, int64_t ldx, const void* base, int64_t ld_base, const void* a,
+                        const void* b, const float* scale, const int32_t* sorted_src, const int32_t* offsets, int T, int n,
+                        int H, int r, int n_slices, const int32_t* widths, void* out, int64_t ld_out, void* workspace,
+                        size_t ws_bytes, void* stream);
+size_t omni_adapter_linear_workspace_bytes(int T, int n, int H, int r, int n_slices);
 
 /*
  * Sort (token, k) assignments by expert.  Replaces torch_npu.npu_moe_init_routing +

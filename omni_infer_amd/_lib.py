@@ -23,6 +23,11 @@ SIGNATURES = {
     "omni_moe_gate_route_workspace_bytes": (c_size_t, [I, I, I]),
     "omni_dynamic_quant": (I, [P, I, c_int64, I, c_int64, P, P, P]),
     "omni_add_rms_norm_quant": (I, [P, P, P, c_int64, I, c_float, P, P, P, P, P]),
+    "omni_sandwich_norm": (I, [P, I, c_int64, P, c_int64, P, P, P, I, c_int64, c_int64, I, c_float, c_float, c_float, P,
+                               c_int64, P, P, P, P]),
+    "omni_swiglu_quant": (I, [P, I, c_int64, c_int64, I, P, P, P, P]),
+    "omni_adapter_linear": (I, [P, I, c_int64, P, c_int64, P, P, P, P, P, I, I, I, I, I, P, P, c_int64, P, c_size_t, P]),
+    "omni_adapter_linear_workspace_bytes": (c_size_t, [I, I, I, I, I]),
     "omni_moe_permute": (I, [P, I, I, I, I, I, P, P, P, P, P, c_size_t, P]),
     "omni_moe_permute_workspace_bytes": (c_size_t, [I, I, I]),
     "omni_moe_group_offsets": (I, [P, I, I, P, P]),
@@ -57,6 +62,7 @@ OMNI_GROUP_MAX, OMNI_GROUP_TOP2SUM = 0, 1
 OMNI_GEMM1_BF16_INTERMEDIATE, OMNI_GEMM1_NO_REQUANT, OMNI_GEMM1_WS_ZEROED = 1, 4, 8
 OMNI_IDX_TOKEN_MAJOR, OMNI_IDX_K_MAJOR = 0, 1
 OMNI_ORDER_SLOT, OMNI_ORDER_K = 0, 1
+OMNI_GATE_NONE, OMNI_GATE_CHANNEL, OMNI_GATE_TOKEN, OMNI_GATE_FULL = 0, 1, 2, 3
 
 OMNI_STATIC_SCRATCH_BYTES = 64 << 20
 ABI_VERSION = 7   # omni_moe_abi_version() of the header these signatures were written from

@@ -555,4 +555,30 @@ inline int placement_tables(const int32_t* pattern, int world, int layers, int e
   return OMNI_OK;
 }
 
+// ------------------------------------------------------------------------------------------------
+// Launch shape of omni_adapter_linear.  The host knows how many tokens and adapters there are, not how the tokens
+// are spread over the adapters, so grids hold the most row tiles there can be.
+// ------------------------------------------------------------------------------------------------
+struct AdapterPlan {
+  int row_tiles;   // 16-row tiles of a block
+  int tiles_max;   // row blocks of the adapters' tokens, at most
+  int ksplit;      // parts of the reduction of the first product
+  int rank_block;  // its columns per block
+  int col_blocks;  // blocks of 64 output columns a block of the second product takes
+};
+inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices) {
+  AdapterPlan p{};
+  const int R = r * n_slices;
+  p.row_tiles = (T >= 1024 && T / 32 >= n && r <= 128) ? 4 : 1;
+  p.tiles_max = T / (16 * p.row_tiles) + imin(n, T);
+  p.rank_block = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
+  const int chunks = (H + 63) / 64;
+  const int64_t blocks = (int64_t)p.tiles_max * ((R + p.rank_block - 1) / p.rank_block);
+  int64_t k = 512 / blocks;
+  if (k > chunks / 8) k = chunks / 8;
+  p.ksplit = k < 1 ? 1 : k > 16 ? 16 : (int)k;
+  p.col_blocks = p.tiles_max > 64 ? 8 : 4;
+  return p;
+}
+
 }  // namespace omni_host

@@ -7,6 +7,7 @@ CPU or eager fallback: tensors must live on the GPU and the library must be buil
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -190,6 +191,165 @@ def add_rms_norm_quant(x: torch.Tensor, residual: Optional[torch.Tensor], weight
             q.view(shape) if q is not None else None, sc.view(shape[:-1]) if sc is not None else None)
 
 
+
+# ----------------------------------------------------------------------------- rows of dense blocks
+def _forward_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The operators have no backward pass: a call that autograd would have to record is refused instead of cutting
+    the graph silently."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: no backward pass is built (call it under torch.no_grad() or detach the inputs)")
+
+
+def _same_device(what: str, x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` [..., cols] as [rows, cols] with elements of a row side by side and rows that do not overlap; a copy
+    only where its strides cannot say that."""
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a [rows, cols] tensor; a single row's stride says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [rows, cols] tensors of one device share an element (columns side by side in one buffer do not)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ea, eb = a.element_size(), b.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    end_a = pa + ((a.shape[0] - 1) * _ld(a) + a.shape[1]) * ea
+    end_b = pb + ((b.shape[0] - 1) * _ld(b) + b.shape[1]) * eb
+    if end_a <= pb or end_b <= pa:
+        return False
+    pitch = _ld(a) * ea
+    if pitch == _ld(b) * eb and a.shape[0] > 1 and b.shape[0] > 1:
+        at = (pb - pa) % pitch
+        return not (at >= a.shape[1] * ea and at + b.shape[1] * eb <= pitch)
+    return True
+
+
+class _on_device:
+    """Makes the device of ``t`` current for a launch, where it is not (the streams and the launch go by the current
+    device)."""
+    __slots__ = ("_guard",)
+
+    def __init__(self, t: torch.Tensor):
+        self._guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor, pre_weight: torch.Tensor,
+                  post_eps: float, pre_eps: float, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
+                  want_y: bool = True, want_quant: bool = False, inplace_residual: bool = False):
+    """The norm after a block, its gate and residual scale, the residual sum and the norm before the next block, in
+    one launch: with ``t = rms_norm(x, post_weight)`` and ``r = residual + residual_scale * gate * t``, returns
+    (rms_norm(r, pre_weight) or None, r, x_int8 or None, pertoken_scale or None), as ``add_rms_norm_quant`` does.
+
+    ``x``, ``residual`` [..., H], the weights [H] and ``gate`` are of one type (bf16, fp16 or fp32).  ``gate`` is [H] (a
+    factor per channel), [..., 1] (per token) or of x's shape.  The sums are fp32 and every output is rounded once: the
+    second norm goes by the unrounded r, the int8 rows by the rounded first result.  A row that holds an infinity or a
+    NaN has it as its scale and zeros as its int8 values.  ``inplace_residual`` writes r over ``residual``."""
+    _need_gpu(x, residual, post_weight, pre_weight, gate)
+    what = "sandwich_norm"
+    _forward_only(what, x, residual, post_weight, pre_weight, gate)
+    dt = x.dtype
+    if dt not in _DT or residual.dtype != dt or post_weight.dtype != dt or pre_weight.dtype != dt or (
+            gate is not None and gate.dtype != dt):
+        raise ValueError(f"{what}: all tensors must be of one type out of bf16, fp16 and fp32")
+    _same_device(what, x, residual, post_weight, pre_weight, gate)
+    if x.dim() == 0:
+        raise ValueError(f"{what}: x must have at least one dimension")
+    shape, H = x.shape, x.shape[-1]
+    if residual.shape != shape:
+        raise ValueError(f"{what}: x and residual differ in shape")
+    if post_weight.shape != (H,) or pre_weight.shape != (H,):
+        raise ValueError(f"{what}: the weights must be [{H}]")
+    x2 = _rows(x, H)
+    rows = x2.shape[0]
+    mode, ldg, g2 = L.OMNI_GATE_NONE, 0, None
+    if gate is not None:
+        if gate.shape == (H,):
+            mode, g2 = L.OMNI_GATE_CHANNEL, gate.contiguous()
+        elif gate.shape == shape:
+            g2 = _rows(gate, H)
+            mode, ldg = L.OMNI_GATE_FULL, _ld(g2)
+        elif gate.dim() == len(shape) and gate.shape == (*shape[:-1], 1):
+            g2 = gate.reshape(-1, 1)
+            g2 = g2.contiguous() if rows > 1 and g2.stride(0) < 1 else g2
+            mode, ldg = L.OMNI_GATE_TOKEN, _ld(g2)
+        else:
+            raise ValueError(f"{what}: the gate must be [{H}], [..., 1] or of x's shape")
+    r2 = _rows(residual, H)
+    if inplace_residual:
+        if r2.data_ptr() != residual.data_ptr():
+            raise ValueError(f"{what}: a residual with these strides cannot be written in place")
+        out, res_out = r2, residual
+        same = x2.data_ptr() == r2.data_ptr() and _ld(x2) == _ld(r2)
+        if (not same and _overlap(x2, out)) or (mode == L.OMNI_GATE_FULL and _overlap(g2, out)):
+            raise ValueError(f"{what}: the residual written in place overlaps another input")
+    else:
+        out = torch.empty(rows, H, dtype=dt, device=x.device)
+        res_out = out.view(shape)
+    y = torch.empty(rows, H, dtype=dt, device=x.device) if want_y else None
+    q = torch.empty(rows, H, dtype=torch.int8, device=x.device) if want_quant else None
+    sc = torch.empty(rows, dtype=torch.float32, device=x.device) if want_quant else None
+    post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
+    with _on_device(x):
+        rc = L.lib().omni_sandwich_norm(_ptr(x2), _DT[dt], _ld(x2), _ptr(r2), _ld(r2), _ptr(post_weight),
+                                        _ptr(pre_weight), _ptr(g2), mode, ldg, rows, H, float(post_eps), float(pre_eps),
+                                        float(residual_scale), _ptr(out), _ld(out), _ptr(y), _ptr(q), _ptr(sc), _stream())
+    L.check(rc, "omni_sandwich_norm")
+    return (y.view(shape) if y is not None else None, res_out, q.view(shape) if q is not None else None,
+            sc.view(shape[:-1]) if sc is not None else None)
+
+
+def swiglu_quant(gate_up: torch.Tensor, want_y: bool = True, want_quant: bool = False):
+    """``silu(gate) * up`` of rows [..., 2I] (gate channels first; bf16, fp16 or fp32), rounded once, and with
+    ``want_quant`` the ``npu_dynamic_quant`` of the rounded result in the same launch.  Returns (h [..., I] or None,
+    x_int8 or None, pertoken_scale or None); a row that holds an infinity or a NaN has it as its scale and zeros as its
+    int8 values."""
+    _need_gpu(gate_up)
+    what = "swiglu_quant"
+    _forward_only(what, gate_up)
+    if gate_up.dtype not in _DT:
+        raise ValueError(f"{what}: unsupported dtype {gate_up.dtype}")
+    if gate_up.dim() == 0 or gate_up.shape[-1] % 2 or gate_up.shape[-1] == 0:
+        raise ValueError(f"{what}: rows must hold a gate and an up half")
+    shape, I = (*gate_up.shape[:-1], gate_up.shape[-1] // 2), gate_up.shape[-1] // 2
+    g2 = _rows(gate_up, 2 * I)
+    rows = g2.shape[0]
+    h = torch.empty(rows, I, dtype=g2.dtype, device=g2.device) if want_y else None
+    q = torch.empty(rows, I, dtype=torch.int8, device=g2.device) if want_quant else None
+    sc = torch.empty(rows, dtype=torch.float32, device=g2.device) if want_quant else None
+    with _on_device(g2):
+        rc = L.lib().omni_swiglu_quant(_ptr(g2), _DT[g2.dtype], _ld(g2), rows, I, _ptr(h), _ptr(q), _ptr(sc), _stream())
+    L.check(rc, "omni_swiglu_quant")
+    return (h.view(shape) if h is not None else None, q.view(shape) if q is not None else None,
+            sc.view(shape[:-1]) if sc is not None else None)
+
+
+def npu_swiglu(x: torch.Tensor) -> torch.Tensor:
+    """Stands in for ``torch_npu.npu_swiglu`` (omni/models/common/layers/activation.py:29)."""
+    return swiglu_quant(x)[0]
+
+
 # ----------------------------------------------------------------------------- permutation
 class Permutation:
     """Result of sorting the (token, k) assignments by local expert."""
@@ -287,6 +447,93 @@ def dense_offsets(M: int, device) -> torch.Tensor:
         t = torch.tensor([0, int(M)], dtype=torch.int32, device=device)
         _DENSE_OFFSETS[key] = t
     return t
+
+
+# ----------------------------------------------------------------------------- adapters
+def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> Permutation:
+    """The tokens of a batch sorted by adapter, for ``adapter_linear``: ``adapter_ids`` [T] integers, the adapter of each
+    token; a value outside [0, n_adapters) (-1, say) means none.  Made once for a batch and used by all its
+    projections."""
+    _need_gpu(adapter_ids)
+    if adapter_ids.dim() != 1 or adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError("adapter_plan: adapter_ids must be [T], int32 or int64")
+    if n_adapters < 1:
+        raise ValueError("adapter_plan: at least one adapter")
+    if adapter_ids.dtype == torch.int64:  # what int32 cannot hold is no adapter either
+        adapter_ids = torch.where((adapter_ids >= 0) & (adapter_ids < n_adapters), adapter_ids, -1)
+    with _on_device(adapter_ids):
+        return moe_permute(adapter_ids.view(-1, 1), 0, int(n_adapters))
+
+
+def _vector_rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``_rows`` for kernels that move 16 bytes at a time: a copy where an alignment forbids that."""
+    t = _rows(t, cols)
+    if t.data_ptr() % 16 or _ld(t) * t.element_size() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Permutation,
+                   scale: Optional[torch.Tensor] = None, slices=None, out: Optional[torch.Tensor] = None,
+                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A shared projection's rows with the low-rank update of each token's adapter:
+    ``out[t] = base[t] + scale[g] * (x[t] @ a[g].T) @ b[g].T`` for the adapter g of token t, ``base[t]`` without one.
+
+    ``x`` [..., H] went into the projection, ``base`` [..., N] came out of it.  ``a`` [n, S*r, H] and ``b`` [n, N, r] hold n
+    adapters; ``slices`` are the S output widths of a stacked projection (gate and up; default: one slice), whose
+    columns take rows j*r..(j+1)*r of ``a``.  ``scale`` [n] fp32 (default 1).  bf16 or fp16; H, r and the widths are
+    multiples of 8, r at most 256 (shorter ranks are filled up with zeros).  ``out`` may be ``base``.  Both products are
+    summed in fp32 and the result is rounded once."""
+    _need_gpu(x, base, a, b, scale)
+    what = "adapter_linear"
+    _forward_only(what, x, base, a, b, scale)
+    dt = x.dtype
+    if dt not in (torch.bfloat16, torch.float16) or base.dtype != dt or a.dtype != dt or b.dtype != dt:
+        raise ValueError(f"{what}: x, base, a and b must be of one type, bf16 or fp16")
+    if a.dim() != 3 or b.dim() != 3 or x.dim() == 0 or base.dim() != x.dim():
+        raise ValueError(f"{what}: x [..., H], base [..., N], a [n, S*r, H] and b [n, N, r]")
+    n, R, H = a.shape
+    N, r = b.shape[1], b.shape[2]
+    widths = (N,) if slices is None else tuple(int(w) for w in slices)
+    if b.shape[0] != n or x.shape[-1] != H or base.shape[-1] != N or x.shape[:-1] != base.shape[:-1]:
+        raise ValueError(f"{what}: x [..., H], base [..., N], a [n, S*r, H] and b [n, N, r] do not fit")
+    if sum(widths) != N or len(widths) * r != R:
+        raise ValueError(f"{what}: slices {widths} do not fit {N} columns and {R} = S * {r} rows of a")
+    if not (a.is_contiguous() and b.is_contiguous()):
+        raise ValueError(f"{what}: a and b must be contiguous")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (n,) or not scale.is_contiguous()):
+        raise ValueError(f"{what}: scale must be a contiguous fp32 [{n}] tensor")
+    x2, base2 = _vector_rows(x, H), _vector_rows(base, N)
+    T = x2.shape[0]
+    if plan.T != T or plan.K != 1 or plan.n_local != n or plan.idx_mode != L.OMNI_IDX_TOKEN_MAJOR:
+        raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n_local} adapters, not {T} and {n}")
+    _same_device(what, x, base, a, b, scale, plan.sorted_src, out, workspace)
+    if out is None:
+        out2 = torch.empty(T, N, dtype=dt, device=x.device)
+        result = out2.view(base.shape)
+    else:
+        if out.dtype != dt or out.shape != base.shape:
+            raise ValueError(f"{what}: out must have base's shape and type")
+        _forward_only(what, out)
+        result, out2 = out, _rows(out, N)
+        if out2.data_ptr() != out.data_ptr() or out2.data_ptr() % 16 or _ld(out2) % 8:
+            raise ValueError(f"{what}: out must have rows of 16-byte aligned, adjacent elements")
+        if out2.data_ptr() == base2.data_ptr() and _ld(out2) != _ld(base2) or (
+                out2.data_ptr() != base2.data_ptr() and _overlap(out2, base2)) or _overlap(out2, x2):
+            raise ValueError(f"{what}: out overlaps an input (it may be base itself)")
+    lib = L.lib()
+    need = lib.omni_adapter_linear_workspace_bytes(T, n, H, r, len(widths))
+    if workspace is None:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+    elif not workspace.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous")
+    with _on_device(x):
+        rc = lib.omni_adapter_linear(_ptr(x2), _DT[dt], _ld(x2), _ptr(base2), _ld(base2), _ptr(a), _ptr(b), _ptr(scale),
+                                     _ptr(plan.sorted_src), _ptr(plan.offsets), T, n, H, r, len(widths),
+                                     (ctypes.c_int32 * len(widths))(*widths), _ptr(out2), _ld(out2), _ptr(workspace),
+                                     workspace.numel() * workspace.element_size(), _stream())
+    L.check(rc, "omni_adapter_linear")
+    return result
 
 
 # ----------------------------------------------------------------------------- weights

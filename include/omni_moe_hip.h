@@ -195,13 +195,14 @@ int omni_swiglu_quant(const void* gate_up, int dtype, int64_t ld, int64_t rows, 
  *   no adapter.
  *   H, r, every width, ldx, ld_base, ld_out multiples of 8, pointers 16-byte aligned; r <= 256, n <= 256, H and N <= 2^20.
  *   out may be base (same stride): rows without an adapter are then left alone.  No other overlap.
- *   workspace: omni_adapter_linear_workspace_bytes(T, n, H, r, n_slices), 16-byte aligned; written and read by this call.
+ *   workspace: omni_adapter_linear_workspace_bytes(T, n, H, r, n_slices, N), 16-byte aligned; written and read by this
+ *   call.  NULL where that is 0.
  */
 int omni_adapter_linear(const void* x, int dtype, int64_t ldx, const void* base, int64_t ld_base, const void* a,
                         const void* b, const float* scale, const int32_t* sorted_src, const int32_t* offsets, int T, int n,
                         int H, int r, int n_slices, const int32_t* widths, void* out, int64_t ld_out, void* workspace,
                         size_t ws_bytes, void* stream);
-size_t omni_adapter_linear_workspace_bytes(int T, int n, int H, int r, int n_slices);
+size_t omni_adapter_linear_workspace_bytes(int T, int n, int H, int r, int n_slices, int N);
 
 /*
  * Sort (token, k) assignments by expert.  Replaces torch_npu.npu_moe_init_routing +

@@ -27,7 +27,7 @@ SIGNATURES = {
                                c_int64, P, P, P, P]),
     "omni_swiglu_quant": (I, [P, I, c_int64, c_int64, I, P, P, P, P]),
     "omni_adapter_linear": (I, [P, I, c_int64, P, c_int64, P, P, P, P, P, I, I, I, I, I, P, P, c_int64, P, c_size_t, P]),
-    "omni_adapter_linear_workspace_bytes": (c_size_t, [I, I, I, I, I]),
+    "omni_adapter_linear_workspace_bytes": (c_size_t, [I, I, I, I, I, I]),
     "omni_moe_permute": (I, [P, I, I, I, I, I, P, P, P, P, P, c_size_t, P]),
     "omni_moe_permute_workspace_bytes": (c_size_t, [I, I, I]),
     "omni_moe_group_offsets": (I, [P, I, I, P, P]),

@@ -560,24 +560,48 @@ inline int placement_tables(const int32_t* pattern, int world, int layers, int e
 // are spread over the adapters, so grids hold the most row tiles there can be.
 // ------------------------------------------------------------------------------------------------
 struct AdapterPlan {
-  int row_tiles;   // 16-row tiles of a block
-  int tiles_max;   // row blocks of the adapters' tokens, at most
-  int ksplit;      // parts of the reduction of the first product
-  int rank_block;  // its columns per block
-  int col_blocks;  // blocks of 64 output columns a block of the second product takes
+  bool fused;         // one launch
+  int waves;          // its wavefronts per block
+  int row_tiles;      // 16-row tiles of a block of the first product: 1, 4, or 8 with the operands in LDS
+  int tiles_max;      // its row blocks, at most
+  int ksplit;         // parts of its reduction
+  int rank_block;     // its columns per block
+  int out_row_tiles;  // 16-row tiles of a block of the second product
+  int out_tiles_max;
+  int unit_blocks;    // blocks of 64 output columns a block of the second product takes
 };
-inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices) {
+inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N) {
   AdapterPlan p{};
-  const int R = r * n_slices;
-  p.row_tiles = (T >= 1024 && T / 32 >= n && r <= 128) ? 4 : 1;
-  p.tiles_max = T / (16 * p.row_tiles) + imin(n, T);
+  const int R = r * n_slices, cols = (N + 63) / 64;
+  // One launch: 16 rows a block.  Its blocks make the first product anew, each reads a slice of A, as often as there are
+  // units of columns.  A compute unit draws about 27 GB/s: 96 KB take it as long as a second launch does.
+  if (r <= 64 && (int64_t)r * H * 2 <= 96 << 10) {
+    const int64_t tiles = T / 16 + imin(n, T) + 1;
+    const int64_t want = 512 / tiles;  // units of columns for two blocks per compute unit
+    const int units = want < 1 ? 1 : want > (cols + 7) / 8 ? (cols + 7) / 8 : (int)want;
+    const int per = (cols + units - 1) / units;
+    if (T < 1024 && tiles * ((int64_t)units * r * H + (int64_t)N * r) * 2 <= (int64_t)64 << 20) {
+      p.fused = true;
+      p.row_tiles = p.out_row_tiles = p.ksplit = 1;
+      p.tiles_max = p.out_tiles_max = T / 16 + imin(n, T);
+      p.rank_block = 64;
+      p.waves = 8;
+      p.unit_blocks = (per + 7) / 8 * 8;
+      return p;
+    }
+  }
+  const bool many = T >= 1024 && T / 32 >= n;
   p.rank_block = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
+  p.row_tiles = !many ? 1 : p.rank_block <= 32 ? 4 : 8;
+  p.tiles_max = T / (16 * p.row_tiles) + imin(n, T);
   const int chunks = (H + 63) / 64;
   const int64_t blocks = (int64_t)p.tiles_max * ((R + p.rank_block - 1) / p.rank_block);
-  int64_t k = 512 / blocks;
+  int64_t k = 512 / blocks;  // two blocks per compute unit
   if (k > chunks / 8) k = chunks / 8;
   p.ksplit = k < 1 ? 1 : k > 16 ? 16 : (int)k;
-  p.col_blocks = p.tiles_max > 64 ? 8 : 4;
+  p.out_row_tiles = many ? 2 : 1;
+  p.out_tiles_max = T / (16 * p.out_row_tiles) + imin(n, T);
+  p.unit_blocks = p.out_tiles_max > 64 ? 16 : 4;
   return p;
 }
 

@@ -193,17 +193,38 @@ def add_rms_norm_quant(x: torch.Tensor, residual: Optional[torch.Tensor], weight
 
 
 # ----------------------------------------------------------------------------- rows of dense blocks
+# The calls below are short on the GPU (a few microseconds for a decode step), so what they ask of torch is counted:
+# the raw handle of the current stream instead of a Stream object, no views where shapes agree, one pass over the checks.
 def _forward_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
     """The operators have no backward pass: a call that autograd would have to record is refused instead of cutting
     the graph silently."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what}: no backward pass is built (call it under torch.no_grad() or detach the inputs)")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what}: no backward pass is built (call it under torch.no_grad() or detach the inputs)")
 
 
-def _same_device(what: str, x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> None:
+def _one_device(what: str, x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> int:
+    """Index of the GPU that holds all of the tensors."""
+    dev = x.device
     for t in tensors:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+        if t is not None and t.device != dev:
+            _need_gpu(t)
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    if not x.is_cuda:
+        _need_gpu(x)
+    return dev.index
+
+
+def _launch(device: int, what: str, fn, *args) -> None:
+    """Calls a library entry on the current stream of ``device``, which is made current where it is not."""
+    if device == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc:
+        L.check(rc, what)
 
 
 def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -211,7 +232,7 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     only where its strides cannot say that."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+    if not t.is_contiguous() and ((cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols)):
         t = t.contiguous()
     return t
 
@@ -238,23 +259,6 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-class _on_device:
-    """Makes the device of ``t`` current for a launch, where it is not (the streams and the launch go by the current
-    device)."""
-    __slots__ = ("_guard",)
-
-    def __init__(self, t: torch.Tensor):
-        self._guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-
-
 def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor, pre_weight: torch.Tensor,
                   post_eps: float, pre_eps: float, gate: Optional[torch.Tensor] = None, residual_scale: float = 1.0,
                   want_y: bool = True, want_quant: bool = False, inplace_residual: bool = False):
@@ -266,22 +270,22 @@ def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Te
     factor per channel), [..., 1] (per token) or of x's shape.  The sums are fp32 and every output is rounded once: the
     second norm goes by the unrounded r, the int8 rows by the rounded first result.  A row that holds an infinity or a
     NaN has it as its scale and zeros as its int8 values.  ``inplace_residual`` writes r over ``residual``."""
-    _need_gpu(x, residual, post_weight, pre_weight, gate)
     what = "sandwich_norm"
+    device = _one_device(what, x, residual, post_weight, pre_weight, gate)
     _forward_only(what, x, residual, post_weight, pre_weight, gate)
     dt = x.dtype
     if dt not in _DT or residual.dtype != dt or post_weight.dtype != dt or pre_weight.dtype != dt or (
             gate is not None and gate.dtype != dt):
         raise ValueError(f"{what}: all tensors must be of one type out of bf16, fp16 and fp32")
-    _same_device(what, x, residual, post_weight, pre_weight, gate)
-    if x.dim() == 0:
+    shape = x.shape
+    if len(shape) == 0:
         raise ValueError(f"{what}: x must have at least one dimension")
-    shape, H = x.shape, x.shape[-1]
+    H = shape[-1]
     if residual.shape != shape:
         raise ValueError(f"{what}: x and residual differ in shape")
     if post_weight.shape != (H,) or pre_weight.shape != (H,):
         raise ValueError(f"{what}: the weights must be [{H}]")
-    x2 = _rows(x, H)
+    x2, r2 = _rows(x, H), _rows(residual, H)
     rows = x2.shape[0]
     mode, ldg, g2 = L.OMNI_GATE_NONE, 0, None
     if gate is not None:
@@ -290,34 +294,35 @@ def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Te
         elif gate.shape == shape:
             g2 = _rows(gate, H)
             mode, ldg = L.OMNI_GATE_FULL, _ld(g2)
-        elif gate.dim() == len(shape) and gate.shape == (*shape[:-1], 1):
+        elif gate.shape == (*shape[:-1], 1):
             g2 = gate.reshape(-1, 1)
             g2 = g2.contiguous() if rows > 1 and g2.stride(0) < 1 else g2
             mode, ldg = L.OMNI_GATE_TOKEN, _ld(g2)
         else:
             raise ValueError(f"{what}: the gate must be [{H}], [..., 1] or of x's shape")
-    r2 = _rows(residual, H)
     if inplace_residual:
         if r2.data_ptr() != residual.data_ptr():
             raise ValueError(f"{what}: a residual with these strides cannot be written in place")
         out, res_out = r2, residual
         same = x2.data_ptr() == r2.data_ptr() and _ld(x2) == _ld(r2)
-        if (not same and _overlap(x2, out)) or (mode == L.OMNI_GATE_FULL and _overlap(g2, out)):
+        if (not same and _overlap(x2, out)) or (mode in (L.OMNI_GATE_TOKEN, L.OMNI_GATE_FULL) and _overlap(g2, out)):
             raise ValueError(f"{what}: the residual written in place overlaps another input")
     else:
-        out = torch.empty(rows, H, dtype=dt, device=x.device)
-        res_out = out.view(shape)
-    y = torch.empty(rows, H, dtype=dt, device=x.device) if want_y else None
-    q = torch.empty(rows, H, dtype=torch.int8, device=x.device) if want_quant else None
-    sc = torch.empty(rows, dtype=torch.float32, device=x.device) if want_quant else None
+        out = torch.empty((rows, H), dtype=dt, device=x.device)
+        res_out = out if len(shape) == 2 else out.view(shape)
+    y = torch.empty((rows, H), dtype=dt, device=x.device) if want_y else None
+    q = sc = None
+    if want_quant:
+        q = torch.empty((rows, H), dtype=torch.int8, device=x.device)
+        sc = torch.empty((rows,), dtype=torch.float32, device=x.device)
     post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
-    with _on_device(x):
-        rc = L.lib().omni_sandwich_norm(_ptr(x2), _DT[dt], _ld(x2), _ptr(r2), _ld(r2), _ptr(post_weight),
-                                        _ptr(pre_weight), _ptr(g2), mode, ldg, rows, H, float(post_eps), float(pre_eps),
-                                        float(residual_scale), _ptr(out), _ld(out), _ptr(y), _ptr(q), _ptr(sc), _stream())
-    L.check(rc, "omni_sandwich_norm")
-    return (y.view(shape) if y is not None else None, res_out, q.view(shape) if q is not None else None,
-            sc.view(shape[:-1]) if sc is not None else None)
+    _launch(device, "omni_sandwich_norm", L.lib().omni_sandwich_norm, x2.data_ptr(), _DT[dt], _ld(x2), r2.data_ptr(), _ld(r2),
+            post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(g2), mode, ldg, rows, H, post_eps, pre_eps, residual_scale,
+            out.data_ptr(), _ld(out), _ptr(y), _ptr(q), _ptr(sc))
+    if len(shape) != 2:
+        y = y.view(shape) if want_y else None
+        q, sc = (q.view(shape), sc.view(shape[:-1])) if want_quant else (None, None)
+    return y, res_out, q, sc
 
 
 def swiglu_quant(gate_up: torch.Tensor, want_y: bool = True, want_quant: bool = False):
@@ -325,24 +330,28 @@ def swiglu_quant(gate_up: torch.Tensor, want_y: bool = True, want_quant: bool = 
     ``want_quant`` the ``npu_dynamic_quant`` of the rounded result in the same launch.  Returns (h [..., I] or None,
     x_int8 or None, pertoken_scale or None); a row that holds an infinity or a NaN has it as its scale and zeros as its
     int8 values."""
-    _need_gpu(gate_up)
     what = "swiglu_quant"
+    device = _one_device(what, gate_up)
     _forward_only(what, gate_up)
-    if gate_up.dtype not in _DT:
-        raise ValueError(f"{what}: unsupported dtype {gate_up.dtype}")
-    if gate_up.dim() == 0 or gate_up.shape[-1] % 2 or gate_up.shape[-1] == 0:
+    dt, shape = gate_up.dtype, gate_up.shape
+    if dt not in _DT:
+        raise ValueError(f"{what}: unsupported dtype {dt}")
+    if len(shape) == 0 or shape[-1] % 2 or shape[-1] == 0:
         raise ValueError(f"{what}: rows must hold a gate and an up half")
-    shape, I = (*gate_up.shape[:-1], gate_up.shape[-1] // 2), gate_up.shape[-1] // 2
+    I = shape[-1] // 2
     g2 = _rows(gate_up, 2 * I)
     rows = g2.shape[0]
-    h = torch.empty(rows, I, dtype=g2.dtype, device=g2.device) if want_y else None
-    q = torch.empty(rows, I, dtype=torch.int8, device=g2.device) if want_quant else None
-    sc = torch.empty(rows, dtype=torch.float32, device=g2.device) if want_quant else None
-    with _on_device(g2):
-        rc = L.lib().omni_swiglu_quant(_ptr(g2), _DT[g2.dtype], _ld(g2), rows, I, _ptr(h), _ptr(q), _ptr(sc), _stream())
-    L.check(rc, "omni_swiglu_quant")
-    return (h.view(shape) if h is not None else None, q.view(shape) if q is not None else None,
-            sc.view(shape[:-1]) if sc is not None else None)
+    h = torch.empty((rows, I), dtype=dt, device=gate_up.device) if want_y else None
+    q = sc = None
+    if want_quant:
+        q = torch.empty((rows, I), dtype=torch.int8, device=gate_up.device)
+        sc = torch.empty((rows,), dtype=torch.float32, device=gate_up.device)
+    _launch(device, "omni_swiglu_quant", L.lib().omni_swiglu_quant, g2.data_ptr(), _DT[dt], _ld(g2), rows, I, _ptr(h), _ptr(q),
+            _ptr(sc))
+    if len(shape) != 2:
+        h = h.view(*shape[:-1], I) if want_y else None
+        q, sc = (q.view(*shape[:-1], I), sc.view(shape[:-1])) if want_quant else (None, None)
+    return h, q, sc
 
 
 def npu_swiglu(x: torch.Tensor) -> torch.Tensor:
@@ -461,7 +470,7 @@ def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> Permutation:
         raise ValueError("adapter_plan: at least one adapter")
     if adapter_ids.dtype == torch.int64:  # what int32 cannot hold is no adapter either
         adapter_ids = torch.where((adapter_ids >= 0) & (adapter_ids < n_adapters), adapter_ids, -1)
-    with _on_device(adapter_ids):
+    with torch.cuda.device(adapter_ids.device):
         return moe_permute(adapter_ids.view(-1, 1), 0, int(n_adapters))
 
 
@@ -471,6 +480,19 @@ def _vector_rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     if t.data_ptr() % 16 or _ld(t) * t.element_size() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
+
+
+_WIDTHS = {}
+
+
+def _widths(slices: tuple):
+    """The C array of a projection's slice widths: a constant of the widths, made once."""
+    arr = _WIDTHS.get(slices)
+    if arr is None:
+        if len(_WIDTHS) > 256:
+            _WIDTHS.clear()
+        arr = _WIDTHS[slices] = (ctypes.c_int32 * len(slices))(*slices)
+    return arr
 
 
 def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Permutation,
@@ -484,20 +506,22 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     columns take rows j*r..(j+1)*r of ``a``.  ``scale`` [n] fp32 (default 1).  bf16 or fp16; H, r and the widths are
     multiples of 8, r at most 256 (shorter ranks are filled up with zeros).  ``out`` may be ``base``.  Both products are
     summed in fp32 and the result is rounded once."""
-    _need_gpu(x, base, a, b, scale)
     what = "adapter_linear"
-    _forward_only(what, x, base, a, b, scale)
+    device = _one_device(what, x, base, a, b, scale, plan.sorted_src if plan is not None else None, out, workspace)
+    _forward_only(what, x, base, a, b, scale, out)
     dt = x.dtype
     if dt not in (torch.bfloat16, torch.float16) or base.dtype != dt or a.dtype != dt or b.dtype != dt:
         raise ValueError(f"{what}: x, base, a and b must be of one type, bf16 or fp16")
-    if a.dim() != 3 or b.dim() != 3 or x.dim() == 0 or base.dim() != x.dim():
+    xs, bs = x.shape, base.shape
+    if a.dim() != 3 or b.dim() != 3 or len(xs) == 0 or len(bs) != len(xs):
         raise ValueError(f"{what}: x [..., H], base [..., N], a [n, S*r, H] and b [n, N, r]")
     n, R, H = a.shape
-    N, r = b.shape[1], b.shape[2]
-    widths = (N,) if slices is None else tuple(int(w) for w in slices)
-    if b.shape[0] != n or x.shape[-1] != H or base.shape[-1] != N or x.shape[:-1] != base.shape[:-1]:
+    nb, N, r = b.shape
+    if nb != n or xs[-1] != H or bs[-1] != N or xs[:-1] != bs[:-1]:
         raise ValueError(f"{what}: x [..., H], base [..., N], a [n, S*r, H] and b [n, N, r] do not fit")
-    if sum(widths) != N or len(widths) * r != R:
+    widths = (N,) if slices is None else tuple(slices)
+    S = len(widths)
+    if sum(widths) != N or S * r != R:
         raise ValueError(f"{what}: slices {widths} do not fit {N} columns and {R} = S * {r} rows of a")
     if not (a.is_contiguous() and b.is_contiguous()):
         raise ValueError(f"{what}: a and b must be contiguous")
@@ -507,33 +531,29 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     T = x2.shape[0]
     if plan.T != T or plan.K != 1 or plan.n_local != n or plan.idx_mode != L.OMNI_IDX_TOKEN_MAJOR:
         raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n_local} adapters, not {T} and {n}")
-    _same_device(what, x, base, a, b, scale, plan.sorted_src, out, workspace)
     if out is None:
-        out2 = torch.empty(T, N, dtype=dt, device=x.device)
-        result = out2.view(base.shape)
+        out2 = torch.empty((T, N), dtype=dt, device=x.device)
+        out = out2 if len(bs) == 2 else out2.view(bs)
     else:
-        if out.dtype != dt or out.shape != base.shape:
+        if out.dtype != dt or out.shape != bs:
             raise ValueError(f"{what}: out must have base's shape and type")
-        _forward_only(what, out)
-        result, out2 = out, _rows(out, N)
+        out2 = _rows(out, N)
         if out2.data_ptr() != out.data_ptr() or out2.data_ptr() % 16 or _ld(out2) % 8:
             raise ValueError(f"{what}: out must have rows of 16-byte aligned, adjacent elements")
         if out2.data_ptr() == base2.data_ptr() and _ld(out2) != _ld(base2) or (
                 out2.data_ptr() != base2.data_ptr() and _overlap(out2, base2)) or _overlap(out2, x2):
             raise ValueError(f"{what}: out overlaps an input (it may be base itself)")
     lib = L.lib()
-    need = lib.omni_adapter_linear_workspace_bytes(T, n, H, r, len(widths))
     if workspace is None:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+        need = lib.omni_adapter_linear_workspace_bytes(T, n, H, r, S, N)
+        if need:
+            workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: the workspace must be contiguous")
-    with _on_device(x):
-        rc = lib.omni_adapter_linear(_ptr(x2), _DT[dt], _ld(x2), _ptr(base2), _ld(base2), _ptr(a), _ptr(b), _ptr(scale),
-                                     _ptr(plan.sorted_src), _ptr(plan.offsets), T, n, H, r, len(widths),
-                                     (ctypes.c_int32 * len(widths))(*widths), _ptr(out2), _ld(out2), _ptr(workspace),
-                                     workspace.numel() * workspace.element_size(), _stream())
-    L.check(rc, "omni_adapter_linear")
-    return result
+    _launch(device, "omni_adapter_linear", lib.omni_adapter_linear, x2.data_ptr(), _DT[dt], _ld(x2), base2.data_ptr(), _ld(base2),
+            a.data_ptr(), b.data_ptr(), _ptr(scale), plan.sorted_src.data_ptr(), plan.offsets.data_ptr(), T, n, H, r, S,
+            _widths(widths), out2.data_ptr(), _ld(out2), _ptr(workspace), 0 if workspace is None else workspace.nbytes)
+    return out
 
 
 # ----------------------------------------------------------------------------- weights

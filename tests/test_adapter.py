@@ -51,10 +51,10 @@ def test_refusals_of_the_library(lib):
     assert call(x=p + 8) == -1 and b"misaligned" in lib.omni_moe_last_error()
     assert call(ldx=68) == -1 and call(src=p + 2) == -1
     assert call(ldo=72) == -1                                    # out is base with another stride
-    assert call(ws_bytes=8) == -3 and call(ws=None) == -3
+    assert call(r=128, ws_bytes=8) == -3 and call(r=128, ws=None) == -3
     assert call(T=0, x=None, ws=None) == 0                       # nothing to do
-    assert lib.omni_adapter_linear_workspace_bytes(0, 2, 64, 16, 1) == 0
-    assert lib.omni_adapter_linear_workspace_bytes(4, 2, 64, 16, 2) >= 4 * 32 * 4
+    assert lib.omni_adapter_linear_workspace_bytes(0, 2, 64, 128, 1, 64) == 0
+    assert lib.omni_adapter_linear_workspace_bytes(4, 2, 64, 128, 2, 64) >= 4 * 256 * 4
 
 
 def test_cpu_tensors_are_refused():
@@ -325,8 +325,10 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="multiple of 8"):
         e = make(4, 2, 8, 60, [8], BF16)
         run(e)
+    e = make(12, 3, 128, 64, [40, 24], BF16)
     with pytest.raises(RuntimeError, match="workspace"):
-        call(workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+        run(e, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    assert torch.equal(run(e, workspace=torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")), run(e))
     with pytest.raises(RuntimeError, match="no backward"):
         call(x=d["x"].clone().requires_grad_())
     with torch.no_grad():

@@ -513,8 +513,9 @@ __global__ __launch_bounds__(256, 4) void adapter_expand_kernel(AdapterArgs g) {
 // Eight wavefronts, 16 sorted rows of one adapter and a unit of columns of one slice.  The first product is made anew by
 // every block of a row block (its operands come from the L2), which saves the launch between the two and the way of v
 // through memory.  The blocks of a row block have numbers 8 apart: they run on one XCD and share its L2.
-template <int DT, int RT, int FUSED_WAVES>
-__global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(AdapterArgs g) {
+constexpr int FUSED_WAVES = 8;
+template <int DT, int RT>
+__global__ __launch_bounds__(FUSED_WAVES * WAVE, RT == 1 ? 4 : RT == 2 ? 3 : 2) void adapter_fused_kernel(AdapterArgs g) {
   constexpr int KP = RT * 16 < 32 ? RT * 16 : (RT * 16 + 31) / 32 * 32, LDK = KP + 8;
   __shared__ float part[FUSED_WAVES][16][RT * 16 + 1];
   __shared__ __align__(16) uint16_t lds[2 * 16 * LDK];
@@ -594,16 +595,10 @@ int launch_adapter(AdapterArgs& g, const omni_host::AdapterPlan& p, hipStream_t 
   g.unit_blocks = p.unit_blocks;
   g.units = column_units(g, p.unit_blocks);
   if (p.fused) {
-    const dim3 grid((unsigned)((p.tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8 * g.units)), block(p.waves * WAVE);
-#define FUSED(RT)                                                                                       \
-  do {                                                                                                  \
-    if (p.waves == 16) hipLaunchKernelGGL((adapter_fused_kernel<DT, RT, 16>), grid, block, 0, st, g);   \
-    else hipLaunchKernelGGL((adapter_fused_kernel<DT, RT, 8>), grid, block, 0, st, g);                  \
-  } while (0)
-    if (g.r <= 16) FUSED(1);
-    else if (g.r <= 32) FUSED(2);
-    else FUSED(4);
-#undef FUSED
+    const dim3 grid((unsigned)((p.tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8 * g.units)), block(FUSED_WAVES * WAVE);
+    if (g.r <= 16) hipLaunchKernelGGL((adapter_fused_kernel<DT, 1>), grid, block, 0, st, g);
+    else if (g.r <= 32) hipLaunchKernelGGL((adapter_fused_kernel<DT, 2>), grid, block, 0, st, g);
+    else hipLaunchKernelGGL((adapter_fused_kernel<DT, 4>), grid, block, 0, st, g);
     OMNI_CHECK_LAUNCH("adapter_linear");
     return OMNI_OK;
   }
@@ -629,10 +624,10 @@ int launch_adapter(AdapterArgs& g, const omni_host::AdapterPlan& p, hipStream_t 
   const size_t shm = (size_t)2 * 16 * p.out_row_tiles * (kp + 8) * 2;
   const dim3 grid2((unsigned)((p.out_tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8), (unsigned)g.units);
 #define EXPAND(MS)                                                                                                   \
-  do {                                                                                                               \
-    if (g.r <= 32) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 1>), grid2, dim3(256), shm, st, g);          \
-    else if (g.r <= 64) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 2>), grid2, dim3(256), shm, st, g);     \
-    else hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 4, 2>), grid2, dim3(256), shm, st, g);                    \
+  do {                                                                                                           \
+    if (g.r <= 32) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 1>), grid2, dim3(256), shm, st, g);      \
+    else if (g.r <= 64) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 2>), grid2, dim3(256), shm, st, g); \
+    else hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 4, 2>), grid2, dim3(256), shm, st, g);                \
   } while (0)
   if (p.out_row_tiles == 1) EXPAND(1);
   else EXPAND(2);

@@ -561,7 +561,6 @@ inline int placement_tables(const int32_t* pattern, int world, int layers, int e
 // ------------------------------------------------------------------------------------------------
 struct AdapterPlan {
   bool fused;         // one launch
-  int waves;          // its wavefronts per block
   int row_tiles;      // 16-row tiles of a block of the first product: 1, 4, or 8 with the operands in LDS
   int tiles_max;      // its row blocks, at most
   int ksplit;         // parts of its reduction
@@ -575,9 +574,9 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
   const int R = r * n_slices, cols = (N + 63) / 64;
   // One launch: 16 rows a block.  Its blocks make the first product anew, each reads a slice of A, as often as there are
   // units of columns.  A compute unit draws about 27 GB/s: 96 KB take it as long as a second launch does.
-  if (r <= 64 && (int64_t)r * H * 2 <= 96 << 10) {
+  if (r <= 64 && (int64_t)r * H * 2 <= 256 << 10) {
     const int64_t tiles = T / 16 + imin(n, T) + 1;
-    const int64_t want = 512 / tiles;  // units of columns for two blocks per compute unit
+    const int64_t want = 256 / tiles;  // units of columns for a block on every compute unit
     const int units = want < 1 ? 1 : want > (cols + 7) / 8 ? (cols + 7) / 8 : (int)want;
     const int per = (cols + units - 1) / units;
     if (T < 1024 && tiles * ((int64_t)units * r * H + (int64_t)N * r) * 2 <= (int64_t)64 << 20) {
@@ -585,7 +584,6 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
       p.row_tiles = p.out_row_tiles = p.ksplit = 1;
       p.tiles_max = p.out_tiles_max = T / 16 + imin(n, T);
       p.rank_block = 64;
-      p.waves = 8;
       p.unit_blocks = (per + 7) / 8 * 8;
       return p;
     }

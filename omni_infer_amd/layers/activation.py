@@ -14,8 +14,7 @@ class SiluAndMul(nn.Module):
     def forward(self, x: Union[Dict[str, Any], torch.Tensor], quant_symbol: bool = False):
         """Quantised input (a dict with ``x_int8``, ``pertoken_scale``, ``out_scale``): the fused
         dequant + SwiGLU + requant (activation.py:15-28), returning ``{x_int8, pertoken_scale}``.
-        A plain bf16 tensor: SwiGLU in fp32 rounded once to bf16 (``npu_swiglu``, :29) -- that
-        branch is outside the W8A8 path and is not built."""
+        A plain tensor: SwiGLU in fp32 rounded once to its type (``npu_swiglu``, :29)."""
         if quant_symbol and isinstance(x, Dict):
             src = x.get("x_int8")
             if not isinstance(src, DeferredInt32Matmul):
@@ -28,4 +27,10 @@ class SiluAndMul(nn.Module):
                                                      None, 0, 1, layer.weight, x.get("out_scale").float().contiguous(),
                                                      offsets, H, I, M)
             return {"x_int8": h, "pertoken_scale": s}
-        raise NotImplementedError("only the W8A8 path is built (bf16 SwiGLU is outside it)")
+        return ops.npu_swiglu(x)
+
+    def forward_rows(self, x: torch.Tensor) -> Dict[str, torch.Tensor]:
+        """Not in the reference: SwiGLU of rows in memory, as rows (``x``, which low-rank adapters read) and quantised
+        for the shared projection (``x_int8``, ``pertoken_scale``), in one launch."""
+        h, x_int8, pertoken_scale = ops.swiglu_quant(x, want_quant=True)
+        return {"x": h, "x_int8": x_int8, "pertoken_scale": pertoken_scale}

@@ -60,7 +60,25 @@ class ReplicatedDeepseekMLP(nn.Module):
         x, _ = self.down_proj.forward(x)
         return x
 
-    def forward(self, x):
+    def enable_adapters(self, max_adapters: int, max_rank: int) -> None:
+        """Room for low-rank adapters beside both projections (``layers/adapters.py``)."""
+        self.gate_up_proj.enable_adapters(max_adapters, max_rank)
+        self.down_proj.enable_adapters(max_adapters, max_rank)
+
+    @property
+    def has_adapters(self) -> bool:
+        return self.gate_up_proj.adapters is not None or self.down_proj.adapters is not None
+
+    def _with_adapters(self, x, adapters):
+        # the products have to lie in memory between the launches: the adapters are added to them
+        gate_up = self.gate_up_proj.forward_rows(x, adapters)
+        h = ops.npu_swiglu(gate_up) if self.down_proj.quant_method is None else self.act_fn_obj.forward_rows(gate_up)
+        return self.down_proj.forward_rows(h, adapters)
+
+    def forward(self, x, adapters=None):
+        """``adapters``: an ``AdapterBatch`` of the tokens' low-rank adapters."""
+        if adapters is not None and self.has_adapters:
+            return self._with_adapters(x, adapters)
         token_num = x.get("x_int8").shape[0] if isinstance(x, Dict) else x.shape[0]
         if token_num > SEQ_SPLIT_LENGTH and not isinstance(x, Dict):  # :105-114
             return torch.concat([self._one(c) for c in x.split(SEQ_SPLIT_LENGTH)])
@@ -163,22 +181,26 @@ class DeepseekMoE(nn.Module):
         return topk_weights, e.apply_expert_load_balance(topk_ids=topk_ids, best_topk_ids=best)
 
     def forward(self, hidden_states: torch.Tensor, residual: torch.Tensor, attn_metadata, layer_id: int = 0,
-                next_attention_weights: Optional[dict] = None):
+                next_attention_weights: Optional[dict] = None, adapters=None):
+        """``adapters``: an ``AdapterBatch`` of the tokens' low-rank adapters; they act on the shared expert (the routed
+        experts have none)."""
+        if self.shared_experts is None or not self.shared_experts.has_adapters:
+            adapters = None
         opt = model_extra_config.operator_opt_config
         allgather_ep = opt.enable_moe_expert_parallel and self.ep_size > 1 and not (
             opt.prefill_dispatch_combine or opt.moe_dispatch_combine)
         same_width = (self.shared_experts is None or
                       self.shared_experts.down_proj.input_size == self.experts.intermediate_size_per_partition)
         if self.fused and allgather_ep and same_width and self.quant_symbol:
-            return self._forward_fused(hidden_states, attn_metadata), residual
+            return self._forward_fused(hidden_states, attn_metadata, adapters), residual
         if isinstance(hidden_states, dict):
             hidden_states = hidden_states["x"]
-        return self._forward_norm_ops(hidden_states, attn_metadata), residual
+        return self._forward_norm_ops(hidden_states, attn_metadata, adapters), residual
 
-    def _forward_norm_ops(self, hidden_states, attn_metadata):
+    def _forward_norm_ops(self, hidden_states, attn_metadata, adapters=None):
         """deepseek_moe.py:243-305 / :307-368 operator by operator, minus the collectives."""
         opt = model_extra_config.operator_opt_config
-        shared_output = self.shared_experts(hidden_states) if self.shared_experts is not None else None
+        shared_output = self.shared_experts(hidden_states, adapters) if self.shared_experts is not None else None
         is_prefill = attn_metadata is None or attn_metadata.prefill is not None
         dispatch = opt.prefill_dispatch_combine if is_prefill else opt.moe_dispatch_combine
         if not dispatch and opt.enable_moe_expert_parallel:
@@ -192,7 +214,17 @@ class DeepseekMoE(nn.Module):
             final = final + shared_output
         return final
 
-    def _forward_fused(self, hidden_states, attn_metadata=None):
+    def _forward_fused(self, hidden_states, attn_metadata=None, adapters=None):
+        if adapters is not None:
+            # the shared expert cannot ride through the grouped launches: its products need the adapters added
+            return self._routed_fused(hidden_states, attn_metadata, None) + self.shared_experts(hidden_states, adapters)
+        shared = None
+        if self.shared_experts is not None:
+            gu, dn = self.shared_experts.gate_up_proj, self.shared_experts.down_proj
+            shared = (gu.weight, gu.weight_scale, dn.weight, dn.weight_scale)
+        return self._routed_fused(hidden_states, attn_metadata, shared)
+
+    def _routed_fused(self, hidden_states, attn_metadata, shared):
         # a dict from RMSNorm.forward_moe_input carries the tokens already quantised
         x_int8 = pertoken_scale = None
         if isinstance(hidden_states, dict):
@@ -200,10 +232,6 @@ class DeepseekMoE(nn.Module):
             hidden_states = hidden_states["x"]
         e = self.experts
         lo = self.global_rank * self._positions_per_rank()
-        shared = None
-        if self.shared_experts is not None:
-            gu, dn = self.shared_experts.gate_up_proj, self.shared_experts.down_proj
-            shared = (gu.weight, gu.weight_scale, dn.weight, dn.weight_scale)
         T, K = hidden_states.shape[0], e.top_k
         E = self.gate.weight.shape[0]
         need = ops.L.lib().omni_moe_w8a8_block_workspace_bytes(T, K, self.local_expert_num, e.hidden_size,

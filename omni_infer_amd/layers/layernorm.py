@@ -52,3 +52,38 @@ class RMSNorm(nn.Module):
         y, residual, x_int8, pertoken_scale = ops.add_rms_norm_quant(
             x, residual, self.weight.data, self.variance_epsilon, want_y=True, want_quant=True)
         return {"x": y, "x_int8": x_int8, "pertoken_scale": pertoken_scale}, residual
+
+
+class SandwichNorm(nn.Module):
+    """Not in the reference: the step from one block to the next of a model that normalises on both sides of its blocks
+    (Pangu-Ultra-MoE's sandwich norm), one launch (omni_sandwich_norm):
+    ``residual = residual + residual_scale * gate * post(x)``, then ``pre(residual)``.
+
+    ``post`` and ``pre`` are the model's own ``RMSNorm`` modules, so parameters keep their names.  ``forward`` takes and
+    returns what ``RMSNorm.forward`` with a residual does, ``quant_symbol`` included.  ``gate``: [hidden_size], [..., 1] or
+    of x's shape."""
+
+    def __init__(self, post: RMSNorm, pre: RMSNorm, residual_scale: float = 1.0):
+        super().__init__()
+        if post.hidden_size != pre.hidden_size:
+            raise ValueError("both norms are of the hidden size")
+        self.post, self.pre, self.residual_scale = post, pre, residual_scale
+
+    def _run(self, x, residual, gate, want_y, want_quant):
+        return ops.sandwich_norm(x, residual, self.post.weight.data, self.pre.weight.data, self.post.variance_epsilon,
+                                 self.pre.variance_epsilon, gate=gate, residual_scale=self.residual_scale, want_y=want_y,
+                                 want_quant=want_quant)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor, gate: Optional[torch.Tensor] = None,
+                quant_symbol: bool = False) -> Union[tuple[dict[str, Any], Any], Any]:
+        quant = bool(model_extra_config.operator_opt_config.use_w8a8_dynamic_quant and quant_symbol)
+        y, residual, x_int8, pertoken_scale = self._run(x, residual, gate, not quant, quant)
+        if quant:
+            return {"x_int8": x_int8, "pertoken_scale": pertoken_scale}, residual
+        return y, residual
+
+    def forward_moe_input(self, x: torch.Tensor, residual: torch.Tensor, gate: Optional[torch.Tensor] = None):
+        """As ``RMSNorm.forward_moe_input``: rows and int8 rows, for ``DeepseekMoE.forward`` and for projections with
+        adapters."""
+        y, residual, x_int8, pertoken_scale = self._run(x, residual, gate, True, True)
+        return {"x": y, "x_int8": x_int8, "pertoken_scale": pertoken_scale}, residual

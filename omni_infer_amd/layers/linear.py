@@ -11,6 +11,8 @@ from typing import List, Optional
 import torch
 import torch.nn as nn
 
+from .adapters import AdapterBatch, AdapterSlots
+
 
 class ReplicatedLinear(nn.Module):
     def __init__(self, input_size: int, output_size: int, bias: bool = False, quant_config=None,
@@ -27,8 +29,39 @@ class ReplicatedLinear(nn.Module):
                                        requires_grad=False)
         else:
             self.quant_method.create_weights(self, [output_size], input_size, self.params_dtype, device=device)
+        self.adapters = None
 
-    def forward(self, x):
+    def enable_adapters(self, max_adapters: int, max_rank: int, dtype: Optional[torch.dtype] = None, device=None) -> None:
+        """Not in the reference: room for low-rank adapters beside the shared weight (``layers/adapters.py``).  They are
+        of the product's type: bf16 for a quantised layer, the weight's for another."""
+        dtype = dtype or (self.params_dtype if self.quant_method is None else torch.bfloat16)
+        self.adapters = AdapterSlots(self.input_size, getattr(self, "output_sizes", [self.output_size]), max_adapters, max_rank,
+                                     dtype, device if device is not None else self.weight.device)
+
+    def forward(self, x, adapters: Optional[AdapterBatch] = None):
+        """``adapters``: the adapters of the batch's tokens; without them, or without ``enable_adapters``, the shared
+        product alone."""
+        if adapters is not None and self.adapters is not None:
+            return self.forward_rows(x, adapters), None
+        return self._shared(x)
+
+    def forward_rows(self, x, adapters: Optional[AdapterBatch] = None) -> torch.Tensor:
+        """The product as rows in memory, also where ``throw_dequant`` leaves it to the activation, with the updates of
+        the tokens' adapters.  ``x``: rows, or a dict of ``x_int8`` and ``pertoken_scale`` with the rows themselves as
+        ``x`` (the adapters read those)."""
+        if self.quant_method is None:
+            x = x["x"] if isinstance(x, dict) else x
+            base, rows = self._shared(x)[0], x
+        else:
+            base = self.quant_method.apply_rows(self, x)
+            rows = x.get("x") if isinstance(x, dict) else x
+        if adapters is not None and self.adapters is not None:
+            if rows is None:
+                raise ValueError("adapters need the rows as they were before their quantisation (key \"x\")")
+            base = self.adapters.add_to(base, rows.to(base.dtype), adapters)
+        return base
+
+    def _shared(self, x):
         if self.quant_method is None:
             if not x.is_cuda:
                 raise RuntimeError("omni_infer_amd operators run on the GPU only (got a CPU tensor)")

@@ -57,16 +57,28 @@ class AscendCompressedTensorsW8A8Int8LinearMethod:
         and its scale together with itself, so that the following ``SiluAndMul`` runs GEMM +
         dequant + SwiGLU + requant as one fused operator (the reference returns the raw int32
         product there, :99-103; the int32 matrix never leaves the chip here)."""
-        if layer.init_state == BEFORE_INIT:
-            layer.init_state = AFTER_INIT
-        if isinstance(x, Dict):
-            x_int8, pertoken_scale = x.get("x_int8"), x.get("pertoken_scale")
-        else:
-            x_int8, pertoken_scale = ops.npu_dynamic_quant(x)
+        x_int8, pertoken_scale = self._quantised(layer, x)
         if bias is not None:
             raise NotImplementedError("bias is not used on the MoE path")
         if getattr(layer, "throw_dequant", False):
             return (DeferredInt32Matmul(x_int8, layer), pertoken_scale)
+        return self._product(layer, x_int8, pertoken_scale)
+
+    def apply_rows(self, layer: torch.nn.Module, x: Union[torch.Tensor, Dict[str, Any]]) -> torch.Tensor:
+        """The bf16 product as rows in memory, also of a layer marked ``throw_dequant``: what a low-rank adapter is
+        added to."""
+        return self._product(layer, *self._quantised(layer, x))
+
+    @staticmethod
+    def _quantised(layer: torch.nn.Module, x: Union[torch.Tensor, Dict[str, Any]]):
+        if layer.init_state == BEFORE_INIT:
+            layer.init_state = AFTER_INIT
+        if isinstance(x, Dict):
+            return x.get("x_int8"), x.get("pertoken_scale")
+        return ops.npu_dynamic_quant(x)
+
+    @staticmethod
+    def _product(layer: torch.nn.Module, x_int8: torch.Tensor, pertoken_scale: torch.Tensor) -> torch.Tensor:
         M = x_int8.shape[0]
         offsets = ops.dense_offsets(M, x_int8.device)
         rows, _ = ops.grouped_gemm2_dequant(x_int8.contiguous(), pertoken_scale.contiguous(), layer.weight,

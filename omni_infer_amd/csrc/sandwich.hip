@@ -34,6 +34,8 @@ __global__ __launch_bounds__(THREADS) void sandwich_norm_kernel(SandwichArgs a) 
   const int H = a.H, nvec = (H + 7) / 8;
   const ET* xr = (const ET*)a.x + r * a.ldx;
   const ET* rr = (const ET*)a.residual + r * a.ldr;
+  const bool wide_gate = a.gate_mode == OMNI_GATE_CHANNEL || a.gate_mode == OMNI_GATE_FULL;
+  const ET* gr = (const ET*)a.gate + (a.gate_mode == OMNI_GATE_FULL ? r * a.ldg : 0);
   float s[MAXV][8], d[MAXV][8];
   float ss = 0.0f;
 #pragma unroll
@@ -57,9 +59,8 @@ __global__ __launch_bounds__(THREADS) void sandwich_norm_kernel(SandwichArgs a) 
       load8<DT, ALIGNED>((const ET*)a.post_w, vi, H, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[i][j] = (s[i][j] * r1) * w[j];
-      if (a.gate_mode == OMNI_GATE_CHANNEL || a.gate_mode == OMNI_GATE_FULL) {
-        const ET* g = (const ET*)a.gate + (a.gate_mode == OMNI_GATE_FULL ? r * a.ldg : 0);
-        load8<DT, ALIGNED>(g, vi, H, w);
+      if (wide_gate) {
+        load8<DT, ALIGNED>(gr, vi, H, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[i][j] = s[i][j] * w[j];
       }
@@ -100,12 +101,20 @@ __global__ __launch_bounds__(THREADS) void sandwich_norm_kernel(SandwichArgs a) 
 
 constexpr int SANDWICH_MAX_H = 16384;
 
+// Few rows (up to two per compute unit): 1024 threads, a vector each, which is 5.3 us for one row of 7168 where 256
+// threads with four each take 7.8, and 6.6 against 9.6 us for 64 rows of 7680 (what is left is the launch, the way to
+// memory and back and the two reductions; weights loaded ahead of them change nothing).  Many rows: 512 threads, 101 us
+// for 8192 rows of 7168 against 111 (256) and 116 us (1024).
 template <int DT, bool ALIGNED>
 int launch_sandwich(const SandwichArgs& a, int64_t rows, hipStream_t st) {
   const dim3 grid((unsigned)rows);
-  if (a.H <= 8 * 256) hipLaunchKernelGGL((sandwich_norm_kernel<DT, 256, 1, ALIGNED>), grid, dim3(256), 0, st, a);
-  else if (a.H <= 8 * 256 * 4) hipLaunchKernelGGL((sandwich_norm_kernel<DT, 256, 4, ALIGNED>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((sandwich_norm_kernel<DT, 1024, 2, ALIGNED>), grid, dim3(1024), 0, st, a);
+#define SANDWICH(THREADS, MAXV) \
+  hipLaunchKernelGGL((sandwich_norm_kernel<DT, THREADS, MAXV, ALIGNED>), grid, dim3(THREADS), 0, st, a)
+  if (a.H <= 8 * 256) SANDWICH(256, 1);
+  else if (a.H > 8 * 1024) SANDWICH(1024, 2);
+  else if (rows <= 512) SANDWICH(1024, 1);
+  else SANDWICH(512, 2);
+#undef SANDWICH
   OMNI_CHECK_LAUNCH("sandwich_norm");
   return OMNI_OK;
 }

@@ -61,12 +61,18 @@ __global__ __launch_bounds__(THREADS) void swiglu_quant_kernel(SwigluArgs a) {
 
 constexpr int SWIGLU_MAX_I = 32768;
 
+// Few rows (up to two per compute unit) of more than 2048: 1024 threads with a vector each, 6.2 us for 64 rows of 8192 with
+// the int8 output where 256 threads with four each take 9.4.  Many rows: 256 threads, 100 us for 8192 rows of 8192
+// (470 MB, 4.7 TB/s) against 103 (512) and 110 us (1024).
 template <int DT, bool ALIGNED>
 int launch_swiglu(const SwigluArgs& a, int64_t rows, hipStream_t st) {
   const dim3 grid((unsigned)rows);
-  if (a.I <= 8 * 256) hipLaunchKernelGGL((swiglu_quant_kernel<DT, 256, 1, ALIGNED>), grid, dim3(256), 0, st, a);
-  else if (a.I <= 8 * 256 * 4) hipLaunchKernelGGL((swiglu_quant_kernel<DT, 256, 4, ALIGNED>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((swiglu_quant_kernel<DT, 1024, 4, ALIGNED>), grid, dim3(1024), 0, st, a);
+#define SWIGLU(THREADS, MAXV) hipLaunchKernelGGL((swiglu_quant_kernel<DT, THREADS, MAXV, ALIGNED>), grid, dim3(THREADS), 0, st, a)
+  if (a.I <= 8 * 256) SWIGLU(256, 1);
+  else if (a.I > 8 * 1024) SWIGLU(1024, 4);
+  else if (rows <= 512) SWIGLU(1024, 1);
+  else SWIGLU(256, 4);
+#undef SWIGLU
   OMNI_CHECK_LAUNCH("swiglu_quant");
   return OMNI_OK;
 }

@@ -206,19 +206,19 @@ def _forward_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 def _one_device(what: str, x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> int:
     """Index of the GPU that holds all of the tensors."""
-    dev = x.device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            _need_gpu(t)
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-    if not x.is_cuda:
+    device = x.get_device()   # -1 on the CPU
+    if device < 0:
         _need_gpu(x)
-    return dev.index
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _need_gpu(t)
+            raise ValueError(f"{what}: tensors on {x.device} and {t.device}")
+    return device
 
 
 def _launch(device: int, what: str, fn, *args) -> None:
     """Calls a library entry on the current stream of ``device``, which is made current where it is not."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -232,9 +232,18 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
     only where its strides cannot say that."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    if not t.is_contiguous() and ((cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols)):
+    if t.is_contiguous():
+        return t
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
         t = t.contiguous()
     return t
+
+
+def _like(t: torch.Tensor, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """New rows without gaps of t's shape."""
+    if t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -308,14 +317,15 @@ def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Te
         if (not same and _overlap(x2, out)) or (mode in (L.OMNI_GATE_TOKEN, L.OMNI_GATE_FULL) and _overlap(g2, out)):
             raise ValueError(f"{what}: the residual written in place overlaps another input")
     else:
-        out = torch.empty((rows, H), dtype=dt, device=x.device)
+        out = _like(x2)
         res_out = out if len(shape) == 2 else out.view(shape)
-    y = torch.empty((rows, H), dtype=dt, device=x.device) if want_y else None
+    y = _like(x2) if want_y else None
     q = sc = None
     if want_quant:
-        q = torch.empty((rows, H), dtype=torch.int8, device=x.device)
+        q = _like(x2, torch.int8)
         sc = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
+    if not (post_weight.is_contiguous() and pre_weight.is_contiguous()):
+        post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
     _launch(device, "omni_sandwich_norm", L.lib().omni_sandwich_norm, x2.data_ptr(), _DT[dt], _ld(x2), r2.data_ptr(), _ld(r2),
             post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(g2), mode, ldg, rows, H, post_eps, pre_eps, residual_scale,
             out.data_ptr(), _ld(out), _ptr(y), _ptr(q), _ptr(sc))
@@ -532,7 +542,7 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     if plan.T != T or plan.K != 1 or plan.n_local != n or plan.idx_mode != L.OMNI_IDX_TOKEN_MAJOR:
         raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n_local} adapters, not {T} and {n}")
     if out is None:
-        out2 = torch.empty((T, N), dtype=dt, device=x.device)
+        out2 = _like(base2)
         out = out2 if len(bs) == 2 else out2.view(bs)
     else:
         if out.dtype != dt or out.shape != bs:

@@ -67,72 +67,93 @@ __device__ __forceinline__ bool find_tile(const AdapterArgs& g, int none, int bm
 }
 
 // ---------------------------------------------------------------- first product
-// Operands of 64 consecutive elements of the reduction: lane l of a wavefront holds row l%16 and the elements 8*(l/16)..+7
-// of either half, so four lanes read 64 consecutive bytes of a row.
-template <int MS, int RT>
-struct ShrinkOps {
-  v4i x[MS][2], a[RT][2];
+// Both products take their operands out of LDS.  An operand of the matrix instruction has another row in every lane of 16,
+// and loads coalesce over neighbouring lanes only: read like that from memory every lane is an access of its own, and a
+// compute unit draws 27 GB/s.  So memory is read 128 bytes of a row by 8 lanes, straight into LDS (lane l of a load writes
+// piece l), and the operands are read from there.  Slot s of row r holds piece s ^ ((r>>1)&7) of the row's eight, applied
+// on the global side: the 16 rows of an operand read then lie on different banks.
+#define OMNI_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+__device__ __forceinline__ void lds_load16(const uint16_t* src, v4i* dst) {
+#if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stubs
+  __builtin_amdgcn_global_load_lds(src, OMNI_LDS_PTR(dst), 16, 0, 0);
+#endif
+}
+// this wavefront's loads into LDS have landed
+__device__ __forceinline__ void lds_landed() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0);
+  asm volatile("" ::: "memory");
+}
+// this wavefront's reads of LDS are done: loads may land on what they read
+__device__ __forceinline__ void lds_read() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0), other counters untouched
+  asm volatile("" ::: "memory");
+}
+
+// Few rows: 16 rows of x and 16*RT of A in a buffer of the wavefront's own, D chunks of 64 elements at a time.
+template <int RT, int D>
+struct Stage {
+  v4i x[D][16 * 8], a[D][RT * 16 * 8];
 };
-template <int MS, int RT>
-__device__ __forceinline__ void shrink_load(ShrinkOps<MS, RT>& o, const uint16_t* const* xp, const uint16_t* const* ap, int k,
-                                            int H, int q) {
+__device__ __forceinline__ constexpr int shrink_depth(int RT) { return RT <= 1 ? 4 : RT <= 2 ? 2 : 1; }
+
+// acc += the chunks [c0, c_end) of 16 rows of x (lane l: row l%16) by 16*RT rows of A
+template <int DT, int RT, int D>
+__device__ __forceinline__ void shrink_chunks(Stage<RT, D>& st, const AdapterArgs& g, const RowBlock& rb, const uint16_t* a, int a_rows,
+                                              int c0, int c_end, v4f* acc) {
+  const int lane = threadIdx.x & (WAVE - 1), m = lane & 15, q = lane >> 4;
+  const uint16_t* xp[2];
+  int px[2], ao[2 * RT], pa[2 * RT];  // a lane's rows of x and A and the first element of its piece
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = min(k + h * 32 + q * 8, H - 8);  // H is a multiple of 8
-#pragma unroll
-    for (int j = 0; j < RT; ++j) o.a[j][h] = *(const v4i*)(ap[j] + at);
-#pragma unroll
-    for (int i = 0; i < MS; ++i) o.x[i][h] = *(const v4i*)(xp[i] + at);
+  for (int i = 0; i < 2; ++i) {
+    const int row = i * 8 + lane / 8;
+    xp[i] = g.x + (size_t)g.sorted_src[rb.row0 + min(row, rb.nrows - 1)] * g.ldx;
+    px[i] = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
   }
-}
-// what lies past the end of the row or of this wavefront's share counts as zero, in both operands: neither may be finite
-template <int MS, int RT>
-__device__ __forceinline__ void shrink_cut(ShrinkOps<MS, RT>& o, int k, int k_end, int q) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const bool in = k + h * 32 + q * 8 < k_end;
-#pragma unroll
-    for (int j = 0; j < RT; ++j) o.a[j][h] = in ? o.a[j][h] : v4i{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < MS; ++i) o.x[i][h] = in ? o.x[i][h] : v4i{0, 0, 0, 0};
+  for (int i = 0; i < 2 * RT; ++i) {
+    const int row = i * 8 + lane / 8;
+    ao[i] = min(row, a_rows - 1) * g.H;
+    pa[i] = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
   }
-}
-template <int DT, int MS, int RT>
-__device__ __forceinline__ void shrink_mac(const ShrinkOps<MS, RT>& o, v4f (*acc)[RT]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < MS; ++i)
-#pragma unroll
-      for (int j = 0; j < RT; ++j) acc[i][j] = mfma_16x16x32<DT>(o.x[i][h], o.a[j][h], acc[i][j]);
-}
-// The chunks [c0, c_end) of 64 elements, D of them requested at a time.  Nothing that is loaded is carried around the
-// loop: the compiler would wait for it there; other wavefronts of the compute unit cover the wait instead.
-template <int DT, int MS, int RT, int D>
-__device__ __forceinline__ void shrink_chunks(const uint16_t* const* xp, const uint16_t* const* ap, int H, int q, int c0, int c_end,
-                                              v4f (*acc)[RT]) {
-  const int k_end = min(c_end * KC, H);
+  const int k_end = min(c_end * KC, g.H), swz = (m >> 1) & 7;
 #pragma unroll 1
   for (int k = c0 * KC; k < k_end; k += D * KC) {
-    ShrinkOps<MS, RT> o[D];
 #pragma unroll
-    for (int d = 0; d < D; ++d) shrink_load<MS, RT>(o[d], xp, ap, k + d * KC, H, q);
-    if (k + D * KC > k_end) {
+    for (int d = 0; d < D; ++d) {
+      const int kd = k + d * KC;  // past the end the last elements come again, and count as zero below
 #pragma unroll
-      for (int d = 0; d < D; ++d) shrink_cut<MS, RT>(o[d], k + d * KC, k_end, q);
+      for (int i = 0; i < 2 * RT; ++i) lds_load16(a + ao[i] + min(kd + pa[i], g.H - 8), st.a[d] + i * WAVE);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) lds_load16(xp[i] + min(kd + px[i], g.H - 8), st.x[d] + i * WAVE);
     }
+    lds_landed();
 #pragma unroll
-    for (int d = 0; d < D; ++d) shrink_mac<DT, MS, RT>(o[d], acc);
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int slot = (h * 4 + q) ^ swz;
+        v4i x = st.x[d][m * 8 + slot], av[RT];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) av[j] = st.a[d][(j * 16 + m) * 8 + slot];
+        if (k + (d + 1) * KC > k_end) {  // zero in both operands: neither may be finite
+          const bool in = k + d * KC + h * 32 + q * 8 < k_end;
+          x = in ? x : v4i{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < RT; ++j) av[j] = in ? av[j] : v4i{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[j] = mfma_16x16x32<DT>(x, av[j], acc[j]);
+      }
+    lds_read();
   }
 }
-__device__ __forceinline__ constexpr int shrink_depth(int MS, int RT) { return MS + RT <= 3 ? 4 : MS + RT <= 5 ? 2 : 1; }
 
 // v = x . A^T for many rows: 128 sorted rows of one adapter by 16*RT of its rows and one part of the reduction.  What bounds
 // it is what a compute unit can draw (27 to 30 GB/s), and A counts there like x, so the eight wavefronts share A: chunks of 64
-// elements go from memory into LDS, 8 rows of a whole cache line an instruction, two stages in turn, two blocks on a
-// compute unit.  Slot s of row r holds piece s ^ ((r>>1)&7) of the row's eight (applied on the global side): the operand
-// reads of 16 rows then fall on different banks.  Wavefronts lie 4 (32 rows each) x 2 (half of the A rows each).
-#define OMNI_LDS_PTR(p) ((__attribute__((address_space(3))) void*)(p))
+// elements go into two stages in turn, two blocks on a compute unit.  Wavefronts lie 4 (32 rows each) x 2 (half of the A rows
+// each).
 constexpr int ST_ROWS = 128, ST_WAVES = 8;
 template <int RT>
 struct TileSrc {
@@ -141,14 +162,10 @@ struct TileSrc {
 };
 template <int RT>
 __device__ __forceinline__ void tile_issue(const TileSrc<RT>& t, int k, int H, int w, v4i* __restrict__ dx, v4i* __restrict__ da) {
-#if defined(__HIP_DEVICE_COMPILE__)  // the host pass only needs the launch stub
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    __builtin_amdgcn_global_load_lds(t.x[i] + min(k + t.px[i], H - 8), OMNI_LDS_PTR(dx + (w * 2 + i) * WAVE), 16, 0, 0);
+  for (int i = 0; i < 2; ++i) lds_load16(t.x[i] + min(k + t.px[i], H - 8), dx + (w * 2 + i) * WAVE);
 #pragma unroll
-  for (int i = 0; i < RT / 4; ++i)
-    __builtin_amdgcn_global_load_lds(t.a[i] + min(k + t.pa[i], H - 8), OMNI_LDS_PTR(da + (w * (RT / 4) + i) * WAVE), 16, 0, 0);
-#endif
+  for (int i = 0; i < RT / 4; ++i) lds_load16(t.a[i] + min(k + t.pa[i], H - 8), da + (w * (RT / 4) + i) * WAVE);
 }
 // all loads of this wavefront into LDS have landed, all its reads are done; then the same holds for the block
 __device__ __forceinline__ void tile_wait() {
@@ -235,47 +252,40 @@ __global__ __launch_bounds__(ST_WAVES * WAVE, 4) void adapter_shrink_tile_kernel
     }
 }
 
-// v = x . A^T.  A block of four wavefronts takes 16*MS sorted rows of one adapter, 16*RT of its rows and one part of
+// v = x . A^T for few rows.  A block of four wavefronts takes 16 sorted rows of one adapter, 16*RT of its rows and one part of
 // the reduction, of which every wavefront has its share.
-template <int DT, int MS, int RT>
+template <int DT, int RT>
 __global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterArgs g) {
-  __shared__ float part[4][16][RT * 16 + 1];
+  constexpr int D = shrink_depth(RT);
+  union Shared {
+    Stage<RT, D> stage[4];
+    float part[4][16][RT * 16 + 1];
+  };
+  __shared__ __align__(16) Shared sh;
   RowBlock rb;
-  if (!find_tile(g, 0, 16 * MS, blockIdx.x, rb)) return;
+  if (!find_tile(g, 0, 16, blockIdx.x, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
   const int c0 = blockIdx.z * RT * 16;
-  const uint16_t* xp[MS];
+  v4f acc[RT];
 #pragma unroll
-  for (int i = 0; i < MS; ++i)
-    xp[i] = g.x + (size_t)g.sorted_src[rb.row0 + min(i * 16 + m, rb.nrows - 1)] * g.ldx;
-  const uint16_t* ap[RT];
-#pragma unroll
-  for (int j = 0; j < RT; ++j)
-    ap[j] = g.a + ((size_t)rb.group * g.R + min(c0 + j * 16 + m, g.R - 1)) * g.H;
-  v4f acc[MS][RT];
-#pragma unroll
-  for (int i = 0; i < MS; ++i)
-#pragma unroll
-    for (int j = 0; j < RT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+  for (int j = 0; j < RT; ++j) acc[j] = v4f{0, 0, 0, 0};
   const int chunks = (g.H + KC - 1) / KC;
   const int per = (chunks + g.ksplit * 4 - 1) / (g.ksplit * 4), c_first = (blockIdx.y * 4 + w) * per;
-  shrink_chunks<DT, MS, RT, shrink_depth(MS, RT)>(xp, ap, g.H, q, c_first, min(chunks, c_first + per), acc);
+  shrink_chunks<DT, RT, D>(sh.stage[w], g, rb, g.a + ((size_t)rb.group * g.R + c0) * g.H, g.R - c0, c_first,
+                           min(chunks, c_first + per), acc);
+  __syncthreads();  // the stages are done with
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh.part[w][q * 4 + e][j * 16 + m] = acc[j][e];
+  __syncthreads();
   float* vp = g.v + (size_t)blockIdx.y * g.T * g.R;
-#pragma unroll
-  for (int i = 0; i < MS; ++i) {
-    if (i) __syncthreads();  // the sums of the rows before have been read
-#pragma unroll
-    for (int j = 0; j < RT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) part[w][q * 4 + e][j * 16 + m] = acc[i][j][e];
-    __syncthreads();
-    for (int t = threadIdx.x; t < 16 * RT * 16; t += 256) {
-      const int row = t / (RT * 16), c = t % (RT * 16);
-      if (i * 16 + row < rb.nrows && c0 + c < g.R)
-        vp[(size_t)(rb.row0 + i * 16 + row) * g.R + c0 + c] =
-            ((part[0][row][c] + part[1][row][c]) + part[2][row][c]) + part[3][row][c];
-    }
+  for (int t = threadIdx.x; t < 16 * RT * 16; t += 256) {
+    const int row = t / (RT * 16), c = t % (RT * 16);
+    if (row < rb.nrows && c0 + c < g.R)
+      vp[(size_t)(rb.row0 + row) * g.R + c0 + c] =
+          ((sh.part[0][row][c] + sh.part[1][row][c]) + sh.part[2][row][c]) + sh.part[3][row][c];
   }
 }
 
@@ -295,127 +305,167 @@ __device__ __forceinline__ void row_power(float mx, float& down, float& up) {
   up = __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// What one wavefront needs for 64 columns of 16*MS rows: the base values and the first 32*NK of B's reduction.
-// Tokens are the columns of the matrix product and output channels its rows, dealt so that a lane ends up with 16
-// channels of token l%16 in two runs of 8 (row 4*q + i of tile t is channel 32*(t/2) + 8*q + 4*(t%2) + i).  Moved like that
-// an instruction would touch half a cache line of 16 rows, which copies at three quarters of the rate of whole lines (64
-// columns of 8192 rows of 4096: 35.6 against 28.0 us); so base and out are moved as whole lines of 8 rows, lane (m, q) with
-// row m%8 (+ 8) and run m/8, and the sums change places with lane m^8.
+// A wavefront takes 64 columns of 16*MS rows at a time.  Tokens are the rows of the matrix product and output channels its
+// columns, dealt so that lane (m, q) ends up with the four channels 4*m..+3 (tile t: channel 4*m + t) of the tokens
+// 16*i + 4*q + e: 16 neighbouring lanes move a whole cache line of base and of out.
 // Ranks up to 16 need one matrix instruction of 32: hi in the first half of the reduction, lo in the second.
-template <int MS, int NK>
-struct ExpandOps {
-  v4i base[MS][2], b[NK][4];  // base[i][h]: row 16*i + 8*h + m%8, columns 32*(m/8) + 8*q ..+7
-};
 struct Columns {
   const uint16_t* b;  // B of the adapter, first row of the slice
   int width, col0, blk, blk_end;
 };
-__device__ __forceinline__ const uint16_t* b_row(const AdapterArgs& g, const Columns& c, int blk, int t, int m) {
-  return c.b + min(blk * NB + (t >> 1) * 32 + (m >> 2) * 8 + (t & 1) * 4 + (m & 3), c.width - 1) * g.r;
+template <int MS>
+struct ExpandOps {
+  v2i base[MS][4];
+};
+// B of 64 channels and up to 64 of the rank (8*P elements a row), in a buffer of the wavefront's own: 64 rows of P pieces of 16
+// bytes one after the other, the piece at place p with the low three bits of its number changed by higher ones, so that
+// the reads of rows 4*m + t fall on different banks.
+__device__ __forceinline__ int panel_place(int unit) {
+  const int x = unit >> 3;
+  return unit ^ ((x ^ (x >> 1) ^ (x >> 2)) & 7);
 }
-// the first of a lane's eight elements of B's reduction
-__device__ __forceinline__ int b_col(const AdapterArgs& g, int k, int q) { return min(g.r <= 16 ? (q & 1) * 8 : k + q * 8, g.r - 8); }
-// No load is conditional (a condition makes the compiler wait for it on the spot): what is past the last row or column
-// repeats the last one and is not stored.
-template <int MS, int NK>
-__device__ __forceinline__ void expand_load(ExpandOps<MS, NK>& o, const AdapterArgs& g, const Columns& c, int blk, const size_t* tok,
-                                            int m, int q) {
+template <int PMAX>
+struct Panel {
+  int row_piece[PMAX];  // what this lane loads: row | piece << 8
+};
+template <int PMAX>
+__device__ __forceinline__ void panel_setup(Panel<PMAX>& pn, int P) {
+  const int lane = threadIdx.x & (WAVE - 1);
 #pragma unroll
-  for (int n = 0; n < NK; ++n)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) o.b[n][t] = *(const v4i*)(b_row(g, c, blk, t, m) + b_col(g, n * 32, q));
-  const int col = c.col0 + min(blk * NB + (m >> 3) * 32 + q * 8, c.width - 8);
-#pragma unroll
-  for (int i = 0; i < MS; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) o.base[i][h] = *(const v4i*)(g.base + tok[i * 2 + h] * g.ldb + col);
-}
-// B past the rank counts as zero: v is zero there, but what was loaded in its place need not be finite
-__device__ __forceinline__ void b_cut(v4i* b, bool in) {
-#pragma unroll
-  for (int t = 0; t < 4; ++t) b[t] = in ? b[t] : v4i{0, 0, 0, 0};
-}
-// the value of lane l^8 (a rotation by 8 inside a row of 16 lanes)
-__device__ __forceinline__ float lane_xor8(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, false));
-}
-template <int DT, int MS>
-__device__ __forceinline__ void expand_mac(v4i* b, bool in, const uint16_t* hi, const uint16_t* lo, int at, int step, v4f (*acc)[4]) {
-  b_cut(b, in);
-#pragma unroll
-  for (int i = 0; i < MS; ++i) {
-    const v4i vh = *(const v4i*)(hi + at + i * step), vl = *(const v4i*)(lo + at + i * step);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      acc[i][t] = mfma_16x16x32<DT>(b[t], vh, acc[i][t]);
-      acc[i][t] = mfma_16x16x32<DT>(b[t], vl, acc[i][t]);
-    }
+  for (int i = 0; i < PMAX; ++i) {
+    const int unit = panel_place(i * WAVE + lane);
+    pn.row_piece[i] = unit / P | (unit % P) << 8;
   }
 }
-template <int DT, int MS, int NK>
-__device__ __forceinline__ void expand_block(ExpandOps<MS, NK>& o, const AdapterArgs& g, const Columns& c, int blk,
-                                             const RowBlock& rb, bool has, const size_t* tok, int m, int q, const uint16_t* hi,
-                                             const uint16_t* lo, int ldk, const float* unscale) {
+template <int PMAX>
+__device__ __forceinline__ void panel_issue(const Panel<PMAX>& pn, int P, const AdapterArgs& g, const Columns& c, int blk, int kc,
+                                            v4i* panel) {
+#pragma unroll
+  for (int i = 0; i < PMAX; ++i) {
+    if (i >= P) break;
+    const int row = min(blk * NB + (pn.row_piece[i] & 255), c.width - 1), k = min(kc + (pn.row_piece[i] >> 8) * 8, g.r - 8);
+    lds_load16(c.b + row * g.r + k, panel + i * WAVE);
+  }
+}
+// No load is conditional (a condition makes the compiler wait for it on the spot): what is past the last row or column
+// repeats the last one and is not stored.
+// `tok` holds the tokens of the rows in LDS: read anew for every block, so that no addresses of rows are kept in registers.
+template <int MS>
+__device__ __forceinline__ void base_load(ExpandOps<MS>& o, const AdapterArgs& g, const Columns& c, int blk, const v4i* tok, int m,
+                                          int q) {
+  const int col = c.col0 + min(blk * NB + m * 4, c.width - 4);
+#pragma unroll
+  for (int i = 0; i < MS; ++i) {
+    const v4i t = tok[i * 4 + q];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.base[i][e] = *(const v2i*)(g.base + (size_t)t[e] * g.ldb + col);
+  }
+}
+// one column block whose panel (the first 64 of the rank) and base values are here or on their way
+template <int DT, int MS, int PMAX>
+__device__ __forceinline__ void expand_block(const ExpandOps<MS>& o, const Panel<PMAX>& pn, int P, v4i* panel, const AdapterArgs& g,
+                                             const Columns& c, int blk, const RowBlock& rb, bool has, const v4i* tok, int m, int q,
+                                             const uint16_t* hi, const uint16_t* lo, int ldk, const float* unscale) {
   v4f acc[MS][4];
 #pragma unroll
   for (int i = 0; i < MS; ++i)
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc[i][t] = v4f{0, 0, 0, 0};
   if (has) {
-    if (NK == 1 && g.r <= 16) {
-      b_cut(o.b[0], (q & 1) * 8 < g.r);
-      const uint16_t* src = ((q >> 1) ? lo : hi) + (q & 1) * 8;
+    lds_landed();
+    if (g.r <= 16) {
+      const int k = (q & 1) * 8;
+      const uint16_t* src = ((q >> 1) ? lo : hi) + k;
+      v4i b[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        b[t] = panel[panel_place((m * 4 + t) * P + min(q & 1, P - 1))];
+        b[t] = k < g.r ? b[t] : v4i{0, 0, 0, 0};  // v is zero there, but what stands in B's place need not be finite
+      }
 #pragma unroll
       for (int i = 0; i < MS; ++i) {
-        const v4i vv = *(const v4i*)(src + (i * 16 + m) * ldk);
+        const v4i v = *(const v4i*)(src + (i * 16 + m) * ldk);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) acc[i][t] = mfma_16x16x32<DT>(o.b[0][t], vv, acc[i][t]);
+        for (int t = 0; t < 4; ++t) acc[i][t] = mfma_16x16x32<DT>(v, b[t], acc[i][t]);
       }
     } else {
+      for (int kc = 0;;) {
 #pragma unroll
-      for (int n = 0; n < NK; ++n)
-        expand_mac<DT, MS>(o.b[n], n * 32 + q * 8 < g.r, hi, lo, m * ldk + n * 32 + q * 8, 16 * ldk, acc);
-      if constexpr (NK > 1) {
-        for (int k = NK * 32; k < g.r; k += 32) {
+        for (int n = 0; n < 2; ++n) {
+          const int k = kc + n * 32;
+          if (k >= g.r) break;
           v4i b[4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) b[t] = *(const v4i*)(b_row(g, c, blk, t, m) + b_col(g, k, q));
-          expand_mac<DT, MS>(b, k + q * 8 < g.r, hi, lo, m * ldk + k + q * 8, 16 * ldk, acc);
+          for (int t = 0; t < 4; ++t) {
+            b[t] = panel[panel_place((m * 4 + t) * P + min(n * 4 + q, P - 1))];
+            b[t] = k + q * 8 < g.r ? b[t] : v4i{0, 0, 0, 0};
+          }
+#pragma unroll
+          for (int i = 0; i < MS; ++i) {
+            const int at = (i * 16 + m) * ldk + k + q * 8;
+            const v4i vh = *(const v4i*)(hi + at), vl = *(const v4i*)(lo + at);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              acc[i][t] = mfma_16x16x32<DT>(vh, b[t], acc[i][t]);
+              acc[i][t] = mfma_16x16x32<DT>(vl, b[t], acc[i][t]);
+            }
+          }
         }
+        kc += 64;
+        if (kc >= g.r) break;
+        lds_read();
+        panel_issue<PMAX>(pn, P, g, c, blk, kc, panel);
+        lds_landed();
       }
     }
   }
-  const int col = blk * NB + (m >> 3) * 32 + q * 8;  // this lane's run
+  const int col = blk * NB + m * 4;
 #pragma unroll
   for (int i = 0; i < MS; ++i) {
-    float un = 1.0f;
-    if constexpr (DT == OMNI_DT_F16) un = has ? unscale[i * 16 + m] : 1.0f;
-    // runs 0 and 1 of token m become run m/8 of the tokens m%8 and m%8 + 8
-    float d[2][8];
+    asm volatile("" ::: "memory");
+    const v4i t = tok[i * 4 + q];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float r0 = acc[i][e / 4][e % 4] * un, r1 = acc[i][2 + e / 4][e % 4] * un;
-      const float other = lane_xor8(m < 8 ? r1 : r0);
-      d[0][e] = m < 8 ? r0 : other;
-      d[1][e] = m < 8 ? other : r1;
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (i * 16 + h * 8 + (m & 7) >= rb.nrows || col >= c.width) continue;  // every lane took part in the exchange
-      v4i v = o.base[i][h];
+    for (int e = 0; e < 4; ++e) {
+      const int row = i * 16 + q * 4 + e;
+      if (row >= rb.nrows || col >= c.width) continue;
+      v2i v = o.base[i][e];
       if (has) {
+        float un = 1.0f;
+        if constexpr (DT == OMNI_DT_F16) un = unscale[row];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const uint32_t u = (uint32_t)o.base[i][h][p];
-          const float v0 = Elem<DT>::cvt((uint16_t)(u & 0xffffu)) + d[h][2 * p];
-          const float v1 = Elem<DT>::cvt((uint16_t)(u >> 16)) + d[h][2 * p + 1];
+        for (int p = 0; p < 2; ++p) {
+          const uint32_t u = (uint32_t)o.base[i][e][p];
+          const float v0 = Elem<DT>::cvt((uint16_t)(u & 0xffffu)) + acc[i][2 * p][e] * un;
+          const float v1 = Elem<DT>::cvt((uint16_t)(u >> 16)) + acc[i][2 * p + 1][e] * un;
           if constexpr (DT == OMNI_DT_BF16) v[p] = (int)f32x2_to_bf16x2(v0, v1);
           else v[p] = (int)((uint32_t)to_elem<DT>(v0) | ((uint32_t)to_elem<DT>(v1) << 16));
         }
       }
-      *(v4i*)(g.out + tok[i * 2 + h] * g.ldo + c.col0 + col) = v;
+      *(v2i*)(g.out + (size_t)t[e] * g.ldo + c.col0 + col) = v;
     }
   }
+}
+// The column blocks of one wavefront.  The first block's panel and base values are on their way when `o` and `blk` come in.
+template <int DT, int MS, int PMAX>
+__device__ __forceinline__ void expand_columns(ExpandOps<MS>& o, const Panel<PMAX>& pn, int P, v4i* panel, const AdapterArgs& g,
+                                               const Columns& c, int blk, int step, const RowBlock& rb, bool has, const v4i* tok,
+                                               int m, int q, const uint16_t* hi, const uint16_t* lo, int ldk, const float* unscale) {
+  for (bool first = true; blk < c.blk_end; blk += step, first = false) {
+    if (!first) {
+      if (has) {
+        lds_read();
+        panel_issue<PMAX>(pn, P, g, c, blk, 0, panel);
+      }
+      base_load<MS>(o, g, c, blk, tok, m, q);
+    }
+    expand_block<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, rb, has, tok, m, q, hi, lo, ldk, unscale);
+  }
+}
+// the tokens of a block's rows; rows past the last repeat it
+template <int MS>
+__device__ __forceinline__ void load_tokens(const AdapterArgs& g, const RowBlock& rb, v4i* tok) {
+  if (threadIdx.x < 16 * MS) ((int*)tok)[threadIdx.x] = g.sorted_src[rb.row0 + min((int)threadIdx.x, rb.nrows - 1)];
+  __syncthreads();
 }
 // which slice and which of its column blocks unit `u` of a launch names; a unit is g.unit_blocks column blocks
 __device__ __forceinline__ Columns find_columns(const AdapterArgs& g, int u, int group, int& slice) {
@@ -434,29 +484,51 @@ __device__ __forceinline__ Columns find_columns(const AdapterArgs& g, int u, int
   return c;
 }
 
+// the parts of a sum in order, U of them requested at a time
+template <int U>
+__device__ __forceinline__ v4f sum_parts(const float* p, size_t step, int n) {
+  v4f s = {0, 0, 0, 0};
+  for (int p0 = 0; p0 < n; p0 += U) {
+    v4f t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) t[u] = *(const v4f*)(p + min(p0 + u, n - 1) * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p0 + u < n) s = s + t[u];
+  }
+  return s;
+}
 // out = base + v . B^T from the sums of the first launch.  A block of four wavefronts takes 16*MS sorted rows and a
 // unit of column blocks; a wavefront takes 64 columns at a time.
-template <int DT, int MS, int KQ, int NK>  // ranks up to 64 * KQ, and up to 32 where NK is 1
-__global__ __launch_bounds__(256, 4) void adapter_expand_kernel(AdapterArgs g) {
-  extern __shared__ __align__(16) uint16_t lds[];  // [2][16*MS][kp + 8]: hi and lo of v, kp = r rounded up to 32 (16)
+template <int DT, int MS, int KQ, int PMAX>  // ranks up to 64 * KQ and, below 64, up to 8 * PMAX
+__global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_expand_kernel(AdapterArgs g) {
+  // [4][64 * P] pieces of B, then [2][16*MS][kp + 8]: hi and lo of v, kp = r rounded up to 32 (16)
+  extern __shared__ __align__(16) v4i dyn[];
+  __shared__ __align__(16) v4i tok[4 * MS];
   __shared__ float unscale[16 * MS];
   RowBlock rb;
   const int none = g.in_place ? 0 : g.T - g.offsets[g.n];
-  if (!find_tile(g, none, 16 * MS, blockIdx.x, rb)) return;
+  const int unit = (int)blockIdx.x / 8 % g.units;  // the units of a row block run one after the other on one XCD
+  if (!find_tile(g, none, 16 * MS, (int)blockIdx.x / 8 / g.units * 8 + (int)blockIdx.x % 8, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
   const bool has = rb.group < g.n;
   int slice;
-  const Columns c = find_columns(g, blockIdx.y, rb.group, slice);
-  size_t tok[MS * 2];
-#pragma unroll
-  for (int i = 0; i < MS * 2; ++i) tok[i] = (size_t)g.sorted_src[rb.row0 + min(i * 8 + (m & 7), rb.nrows - 1)];
-  ExpandOps<MS, NK> o;
-  int blk = c.blk + w;
-  if (blk < c.blk_end) expand_load<MS, NK>(o, g, c, blk, tok, m, q);  // on its way while v is made
+  const Columns c = find_columns(g, unit, rb.group, slice);
+  const int P = min(g.r, 64) / 8;
+  v4i* panel = dyn + w * WAVE * P;
+  Panel<PMAX> pn;
+  panel_setup<PMAX>(pn, P);
+  load_tokens<MS>(g, rb, tok);
+  ExpandOps<MS> o;
+  const int blk = c.blk + w;
+  if (blk < c.blk_end) {  // on its way while v is made
+    if (has) panel_issue<PMAX>(pn, P, g, c, blk, 0, panel);
+    base_load<MS>(o, g, c, blk, tok, m, q);
+  }
   const int kp = g.r <= 16 ? 16 : (g.r + 31) / 32 * 32, ldk = kp + 8;
-  uint16_t* hi = lds;
-  uint16_t* lo = lds + 16 * MS * ldk;
+  uint16_t* hi = (uint16_t*)(dyn + 4 * WAVE * P);
+  uint16_t* lo = hi + 16 * MS * ldk;
   if (has) {
     const float sc = g.scale ? g.scale[rb.group] : 1.0f;
     const size_t part = (size_t)g.T * g.R;
@@ -471,15 +543,7 @@ __global__ __launch_bounds__(256, 4) void adapter_expand_kernel(AdapterArgs g) {
       for (int j = 0; j < KQ; ++j) {
         const int k = (j * 16 + l) * 4;
         const float* p = vr + min(k, g.r - 4);
-        v4f s = {0, 0, 0, 0};
-        for (int p0 = 0; p0 < g.ksplit; p0 += 4) {
-          v4f t[4];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) t[u] = *(const v4f*)(p + min(p0 + u, g.ksplit - 1) * part);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (p0 + u < g.ksplit) s = s + t[u];
-        }
+        const v4f s = g.ksplit > 4 ? sum_parts<8>(p, part, g.ksplit) : sum_parts<4>(p, part, g.ksplit);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           v[j][e] = k < g.r ? s[e] * sc : 0.0f;
@@ -502,11 +566,7 @@ __global__ __launch_bounds__(256, 4) void adapter_expand_kernel(AdapterArgs g) {
     }
     __syncthreads();
   }
-  if (blk < c.blk_end) expand_block<DT, MS, NK>(o, g, c, blk, rb, has, tok, m, q, hi, lo, ldk, unscale);
-  for (blk += 4; blk < c.blk_end; blk += 4) {
-    expand_load<MS, NK>(o, g, c, blk, tok, m, q);
-    expand_block<DT, MS, NK>(o, g, c, blk, rb, has, tok, m, q, hi, lo, ldk, unscale);
-  }
+  expand_columns<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, 4, rb, has, tok, m, q, hi, lo, ldk, unscale);
 }
 
 // ---------------------------------------------------------------- both products in one launch
@@ -515,10 +575,16 @@ __global__ __launch_bounds__(256, 4) void adapter_expand_kernel(AdapterArgs g) {
 // through memory.  The blocks of a row block have numbers 8 apart: they run on one XCD and share its L2.
 constexpr int FUSED_WAVES = 8;
 template <int DT, int RT>
-__global__ __launch_bounds__(FUSED_WAVES * WAVE, RT == 1 ? 4 : RT == 2 ? 3 : 2) void adapter_fused_kernel(AdapterArgs g) {
-  constexpr int KP = RT * 16 < 32 ? RT * 16 : (RT * 16 + 31) / 32 * 32, LDK = KP + 8;
-  __shared__ float part[FUSED_WAVES][16][RT * 16 + 1];
+__global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(AdapterArgs g) {
+  constexpr int KP = RT * 16 < 32 ? RT * 16 : (RT * 16 + 31) / 32 * 32, LDK = KP + 8, D = shrink_depth(RT), PMAX = 2 * RT;
+  union Shared {
+    Stage<RT, D> stage[FUSED_WAVES];
+    float part[FUSED_WAVES][16][RT * 16 + 1];
+  };
+  __shared__ __align__(16) Shared sh;
+  __shared__ __align__(16) v4i panels[FUSED_WAVES][WAVE * PMAX];
   __shared__ __align__(16) uint16_t lds[2 * 16 * LDK];
+  __shared__ __align__(16) v4i tok[4];
   __shared__ float unscale[16];
   const int none = g.in_place ? 0 : g.T - g.offsets[g.n];
   const int unit = (int)blockIdx.x / 8 % g.units;
@@ -529,28 +595,30 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE, RT == 1 ? 4 : RT == 2 ? 3 : 2) 
   const bool has = rb.group < g.n;
   int slice;
   const Columns c = find_columns(g, unit, rb.group, slice);
-  const size_t tok[2] = {(size_t)g.sorted_src[rb.row0 + min(m & 7, rb.nrows - 1)],
-                         (size_t)g.sorted_src[rb.row0 + min(8 + (m & 7), rb.nrows - 1)]};
-  constexpr int NK = RT > 2 ? 2 : 1;
-  ExpandOps<1, NK> o;
-  int blk = c.blk + w;
-  if (blk < c.blk_end) expand_load<1, NK>(o, g, c, blk, tok, m, q);  // on its way during the first product
+  const int P = g.r / 8;
+  v4i* panel = panels[w];
+  Panel<PMAX> pn;
+  panel_setup<PMAX>(pn, P);
+  load_tokens<1>(g, rb, tok);
+  ExpandOps<1> o;
+  const int blk = c.blk + w;
+  if (blk < c.blk_end) {  // on its way during the first product
+    if (has) panel_issue<PMAX>(pn, P, g, c, blk, 0, panel);
+    base_load<1>(o, g, c, blk, tok, m, q);
+  }
   if (has) {
     const float sc = g.scale ? g.scale[rb.group] : 1.0f;
-    const uint16_t* xp[1] = {g.x + (m < 8 ? tok[0] : tok[1]) * g.ldx};
-    const uint16_t* ap[RT];
+    v4f acc[RT];
 #pragma unroll
-    for (int j = 0; j < RT; ++j)
-      ap[j] = g.a + ((size_t)rb.group * g.R + slice * g.r + min(j * 16 + m, g.r - 1)) * g.H;
-    v4f acc[1][RT];
-#pragma unroll
-    for (int j = 0; j < RT; ++j) acc[0][j] = v4f{0, 0, 0, 0};
+    for (int j = 0; j < RT; ++j) acc[j] = v4f{0, 0, 0, 0};
     const int chunks = (g.H + KC - 1) / KC, per = (chunks + FUSED_WAVES - 1) / FUSED_WAVES;
-    shrink_chunks<DT, 1, RT, shrink_depth(1, RT)>(xp, ap, g.H, q, w * per, min(chunks, (w + 1) * per), acc);
+    shrink_chunks<DT, RT, D>(sh.stage[w], g, rb, g.a + ((size_t)rb.group * g.R + slice * g.r) * g.H, g.r, w * per,
+                             min(chunks, (w + 1) * per), acc);
+    __syncthreads();  // the stages are done with
 #pragma unroll
     for (int j = 0; j < RT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[w][q * 4 + e][j * 16 + m] = acc[0][j][e];
+      for (int e = 0; e < 4; ++e) sh.part[w][q * 4 + e][j * 16 + m] = acc[j][e];
     __syncthreads();
     if (threadIdx.x < 256) {  // a row by 16 lanes
       const int row = threadIdx.x / 16, l = threadIdx.x % 16;
@@ -559,9 +627,9 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE, RT == 1 ? 4 : RT == 2 ? 3 : 2) 
       for (int j = 0; j < KP / 16; ++j) {
         v[j] = 0.0f;
         if (j < RT && j * 16 + l < g.r) {
-          float s = part[0][row][j * 16 + l];
+          float s = sh.part[0][row][j * 16 + l];
 #pragma unroll
-          for (int p = 1; p < FUSED_WAVES; ++p) s = s + part[p][row][j * 16 + l];
+          for (int p = 1; p < FUSED_WAVES; ++p) s = s + sh.part[p][row][j * 16 + l];
           v[j] = s * sc;
           if (fabsf(v[j]) < __builtin_inff()) mx = fmaxf(mx, fabsf(v[j]));
         }
@@ -577,11 +645,7 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE, RT == 1 ? 4 : RT == 2 ? 3 : 2) 
     }
     __syncthreads();
   }
-  if (blk < c.blk_end) expand_block<DT, 1, NK>(o, g, c, blk, rb, has, tok, m, q, lds, lds + 16 * LDK, LDK, unscale);
-  for (blk += FUSED_WAVES; blk < c.blk_end; blk += FUSED_WAVES) {
-    expand_load<1, NK>(o, g, c, blk, tok, m, q);
-    expand_block<DT, 1, NK>(o, g, c, blk, rb, has, tok, m, q, lds, lds + 16 * LDK, LDK, unscale);
-  }
+  expand_columns<DT, 1, PMAX>(o, pn, P, panel, g, c, blk, FUSED_WAVES, rb, has, tok, m, q, lds, lds + 16 * LDK, LDK, unscale);
 }
 
 int column_units(const AdapterArgs& g, int unit_blocks) {
@@ -602,32 +666,29 @@ int launch_adapter(AdapterArgs& g, const omni_host::AdapterPlan& p, hipStream_t 
     OMNI_CHECK_LAUNCH("adapter_linear");
     return OMNI_OK;
   }
-#define SHRINK(MS, RT) hipLaunchKernelGGL((adapter_shrink_kernel<DT, MS, RT>), grid, dim3(256), 0, st, g)
-#define SHRINK_RT(MS)                       \
-  do {                                      \
-    if (p.rank_block == 16) SHRINK(MS, 1);  \
-    else if (p.rank_block == 32) SHRINK(MS, 2); \
-    else if (p.rank_block == 64) SHRINK(MS, 4); \
-    else SHRINK(MS, 8);                     \
-  } while (0)
+#define SHRINK(RT) hipLaunchKernelGGL((adapter_shrink_kernel<DT, RT>), grid, dim3(256), 0, st, g)
+#define SHRINK_TILE(RT) hipLaunchKernelGGL((adapter_shrink_tile_kernel<DT, RT>), grid, dim3(ST_WAVES * WAVE), 0, st, g)
   const dim3 grid((unsigned)((p.tiles_max + 7) / 8 * 8), (unsigned)p.ksplit, (unsigned)((g.R + p.rank_block - 1) / p.rank_block));
-  if (p.row_tiles == 1) SHRINK_RT(1);
-  else if (p.row_tiles == 4) {
-    if (p.rank_block == 16) SHRINK(4, 1);
-    else SHRINK(4, 2);
-  } else if (p.rank_block == 64) hipLaunchKernelGGL((adapter_shrink_tile_kernel<DT, 4>), grid, dim3(ST_WAVES * WAVE), 0, st, g);
-  else hipLaunchKernelGGL((adapter_shrink_tile_kernel<DT, 8>), grid, dim3(ST_WAVES * WAVE), 0, st, g);
-#undef SHRINK_RT
+  if (p.row_tiles == 8) {
+    if (p.rank_block == 64) SHRINK_TILE(4);
+    else SHRINK_TILE(8);
+  } else {
+    if (p.rank_block == 16) SHRINK(1);
+    else if (p.rank_block == 32) SHRINK(2);
+    else if (p.rank_block == 64) SHRINK(4);
+    else SHRINK(8);
+  }
+#undef SHRINK_TILE
 #undef SHRINK
   OMNI_CHECK_LAUNCH("adapter_linear");
   const int kp = g.r <= 16 ? 16 : (g.r + 31) / 32 * 32;
-  const size_t shm = (size_t)2 * 16 * p.out_row_tiles * (kp + 8) * 2;
-  const dim3 grid2((unsigned)((p.out_tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8), (unsigned)g.units);
+  const size_t shm = (size_t)4 * WAVE * (g.r < 64 ? g.r / 8 : 8) * 16 + (size_t)2 * 16 * p.out_row_tiles * (kp + 8) * 2;
+  const dim3 grid2((unsigned)((p.out_tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8 * g.units));
 #define EXPAND(MS)                                                                                                   \
   do {                                                                                                           \
-    if (g.r <= 32) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 1>), grid2, dim3(256), shm, st, g);      \
-    else if (g.r <= 64) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 2>), grid2, dim3(256), shm, st, g); \
-    else hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 4, 2>), grid2, dim3(256), shm, st, g);                \
+    if (g.r <= 32) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 4>), grid2, dim3(256), shm, st, g);      \
+    else if (g.r <= 64) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 8>), grid2, dim3(256), shm, st, g); \
+    else hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 4, 8>), grid2, dim3(256), shm, st, g);                \
   } while (0)
   if (p.out_row_tiles == 1) EXPAND(1);
   else EXPAND(2);

@@ -561,7 +561,7 @@ inline int placement_tables(const int32_t* pattern, int world, int layers, int e
 // ------------------------------------------------------------------------------------------------
 struct AdapterPlan {
   bool fused;         // one launch
-  int row_tiles;      // 16-row tiles of a block of the first product: 1, 4, or 8 with the operands in LDS
+  int row_tiles;      // 16-row tiles of a block of the first product: 1, or 8 with the operands in LDS
   int tiles_max;      // its row blocks, at most
   int ksplit;         // parts of its reduction
   int rank_block;     // its columns per block
@@ -573,7 +573,10 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
   AdapterPlan p{};
   const int R = r * n_slices, cols = (N + 63) / 64;
   // One launch: 16 rows a block.  Its blocks make the first product anew, each reads a slice of A, as often as there are
-  // units of columns.  A compute unit draws about 27 GB/s: 96 KB take it as long as a second launch does.
+  // units of columns.  Measured on the GPU: 8.5 us against 7.7 us in two launches for one token (rank 16, 7168 -> 2 x 2048),
+  // 11.2 against 14.2 us for 64 tokens with 64 adapters (rank 16, 2048 -> 7168), 8.3 against 9.9 us for 333 tokens with 12
+  // (rank 24, 1992 -> 1048); called from Python, where a launch costs the host 3 us and the workspace another, 11.5 against
+  // 16.5 us.  A slice of 256 KB and 64 MB over all blocks are where one launch stops paying.
   if (r <= 64 && (int64_t)r * H * 2 <= 256 << 10) {
     const int64_t tiles = T / 16 + imin(n, T) + 1;
     const int64_t want = 256 / tiles;  // units of columns for a block on every compute unit
@@ -589,15 +592,15 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
     }
   }
   const bool many = T >= 1024 && T / 32 >= n;
-  p.rank_block = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
-  p.row_tiles = !many ? 1 : p.rank_block <= 32 ? 4 : 8;
+  p.rank_block = R <= 16 && !many ? 16 : R <= 32 && !many ? 32 : R <= 64 ? 64 : 128;
+  p.row_tiles = many ? 8 : 1;
   p.tiles_max = T / (16 * p.row_tiles) + imin(n, T);
   const int chunks = (H + 63) / 64;
   const int64_t blocks = (int64_t)p.tiles_max * ((R + p.rank_block - 1) / p.rank_block);
   int64_t k = 512 / blocks;  // two blocks per compute unit
   if (k > chunks / 8) k = chunks / 8;
   p.ksplit = k < 1 ? 1 : k > 16 ? 16 : (int)k;
-  p.out_row_tiles = many ? 2 : 1;
+  p.out_row_tiles = many && r > 32 && r <= 128 ? 2 : 1;  // what the second product keeps in LDS stays below 64 KB
   p.out_tiles_max = T / (16 * p.out_row_tiles) + imin(n, T);
   p.unit_blocks = p.out_tiles_max > 64 ? 16 : 4;
   return p;

@@ -23,7 +23,7 @@ int main() {
     const int T = it % 3 ? pick(1, 200) : pick(1, 20000), n = pick(1, it % 2 ? 8 : 256);
     const int H = 8 * pick(1, it % 5 ? 200 : 2000), r = 8 * pick(1, 32), S = pick(1, 4), N = 8 * pick(1, 2000);
     const omni_host::AdapterPlan p = omni_host::adapter_plan(T, n, H, r, S, N);
-    CHECK(p.row_tiles == 1 || (p.row_tiles == 4 && p.rank_block <= 32) || (p.row_tiles == 8 && p.rank_block >= 64));
+    CHECK(p.row_tiles == 1 || (p.row_tiles == 8 && p.rank_block >= 64));
     CHECK(p.out_row_tiles == 1 || p.out_row_tiles == 2);
     CHECK(!p.fused || (r <= 64 && p.row_tiles == 1 && p.out_row_tiles == 1 && p.ksplit == 1));
     CHECK(p.ksplit >= 1 && p.ksplit <= 16 && p.unit_blocks >= 1);

@@ -149,6 +149,9 @@ CASES = [  # T, n, r, H, widths
     (2047, 2, 8, 64, [40]),
     (1100, 2, 128, 192, [328]),
     (1030, 1, 72, 4104, [64, 72]),
+    (1300, 2, 256, 328, [200]),
+    (1025, 3, 40, 4096, [128, 24]),
+    (33, 2, 56, 136, [200]),
 ]
 
 

@@ -25,9 +25,9 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 constexpr int MAX_SLICES = 4;
 constexpr int MAX_RANK = 256;
 constexpr int MAX_ADAPTERS = 256;
-constexpr int MAX_WIDTH = 1 << 20, MAX_TOKENS = 1 << 24;  // what the grids hold
-constexpr int KC = 64;        // elements of the reduction a wavefront takes at a time: two matrix instructions
-constexpr int NB = 64;        // output columns a wavefront takes at a time
+constexpr int MAX_WIDTH = 1 << 20, MAX_TOKENS = 1 << 24, MAX_BLOCKS = 1 << 23;  // what indexes and grids hold
+constexpr int KC = 64;  // elements of the reduction a wavefront takes at a time: two matrix instructions
+constexpr int NB = 64;  // output columns a wavefront takes at a time
 
 struct AdapterArgs {
   const uint16_t *x, *base, *a, *b;
@@ -151,9 +151,10 @@ __device__ __forceinline__ void shrink_chunks(Stage<RT, D>& st, const AdapterArg
 }
 
 // v = x . A^T for many rows: 128 sorted rows of one adapter by 16*RT of its rows and one part of the reduction.  What bounds
-// it is what a compute unit can draw (27 to 30 GB/s), and A counts there like x, so the eight wavefronts share A: chunks of 64
-// elements go into two stages in turn, two blocks on a compute unit.  Wavefronts lie 4 (32 rows each) x 2 (half of the A rows
-// each).
+// it is what a compute unit can draw from behind its cache (27 to 30 GB/s), and A counts there like x, so the eight
+// wavefronts share A: chunks of 64 elements go into two stages in turn, two blocks on a compute unit.  Wavefronts lie 4 (32
+// rows each) x 2 (half of the A rows each).  8192 x 7168 tokens by 128 rows of A in 35 to 41 us (117 MB of x, 3 TB/s), where
+// 64 rows a block with operands straight from memory took 72; 8192 x 2048 by 16 rows in 12 us.
 constexpr int ST_ROWS = 128, ST_WAVES = 8;
 template <int RT>
 struct TileSrc {
@@ -499,7 +500,10 @@ __device__ __forceinline__ v4f sum_parts(const float* p, size_t step, int n) {
   return s;
 }
 // out = base + v . B^T from the sums of the first launch.  A block of four wavefronts takes 16*MS sorted rows and a
-// unit of column blocks; a wavefront takes 64 columns at a time.
+// unit of column blocks; a wavefront takes 64 columns at a time.  Bound by base and out, which a plain copy moves in 26 us for
+// 8192 rows of 2 x 2048 and in 45 to 49 us for 8192 of 7168: 51 us at rank 64 (MS = 2; B, read by every block from the L2, is
+// as much again) and 55 us at rank 16 (MS = 1: more wavefronts; MS = 2 takes 61).  16 column blocks a unit: 32
+// take 56 and 62 us.
 template <int DT, int MS, int KQ, int PMAX>  // ranks up to 64 * KQ and, below 64, up to 8 * PMAX
 __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_expand_kernel(AdapterArgs g) {
   // [4][64 * P] pieces of B, then [2][16*MS][kp + 8]: hi and lo of v, kp = r rounded up to 32 (16)
@@ -573,6 +577,8 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
 // Eight wavefronts, 16 sorted rows of one adapter and a unit of columns of one slice.  The first product is made anew by
 // every block of a row block (its operands come from the L2), which saves the launch between the two and the way of v
 // through memory.  The blocks of a row block have numbers 8 apart: they run on one XCD and share its L2.
+// Bound by latency: the launch and a chain of four trips to memory.  One token, rank 16, 7168 -> 2 x 2048: 8.5 us.  64 tokens
+// with 64 adapters, rank 16, 2048 -> 7168: 11.1 us for 21 MB.
 constexpr int FUSED_WAVES = 8;
 template <int DT, int RT>
 __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(AdapterArgs g) {
@@ -737,6 +743,8 @@ extern "C" int omni_adapter_linear(const void* x, int dtype, int64_t ldx, const 
     OMNI_FAIL(OMNI_E_INVALID, "adapter_linear: misaligned pointer or row stride");
   if (out == base && ld_out != ld_base) OMNI_FAIL(OMNI_E_INVALID, "adapter_linear: out is base with another row stride");
   const omni_host::AdapterPlan p = omni_host::adapter_plan(T, n, H, r, n_slices, (int)N);
+  if (((int64_t)p.out_tiles_max + 8) * (N / 64 / p.unit_blocks + n_slices) > MAX_BLOCKS)
+    OMNI_FAIL(OMNI_E_UNSUPPORTED, "adapter_linear: %d tokens of %lld columns", T, (long long)N);
   const size_t need = omni_adapter_linear_workspace_bytes(T, n, H, r, n_slices, (int)N);
   if (need && (ws_bytes < need || !workspace)) OMNI_FAIL(OMNI_E_WORKSPACE, "adapter_linear: workspace %zu < %zu", workspace ? ws_bytes : 0, need);
   if ((uintptr_t)workspace % 16) OMNI_FAIL(OMNI_E_INVALID, "adapter_linear: misaligned workspace");

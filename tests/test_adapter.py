@@ -45,6 +45,7 @@ def test_refusals_of_the_library(lib):
     assert call(widths=(ctypes.c_int32 * 1)(60)) == -2 and b"multiple of 8" in lib.omni_moe_last_error()
     assert call(H=60) == -2 and call(r=12) == -2 and call(r=264) == -2 and call(n=257) == -2
     assert call(T=(1 << 24) + 1) == -2
+    assert call(T=1 << 24, widths=(ctypes.c_int32 * 1)(1 << 20), ldb=1 << 20, ldo=1 << 20) == -2    # more blocks than a grid holds
     assert call(ldx=56) == -1 and call(ldb=56) == -1 and call(ldo=56) == -1
     for null in ("x", "base", "a", "b", "src", "off", "out"):
         assert call(**{null: None}) == -1

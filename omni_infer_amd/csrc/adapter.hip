@@ -78,7 +78,7 @@ __device__ __forceinline__ void lds_load16(const uint16_t* src, v4i* dst) {
   __builtin_amdgcn_global_load_lds(src, OMNI_LDS_PTR(dst), 16, 0, 0);
 #endif
 }
-// this wavefront's loads into LDS have landed
+// this wavefront's loads into LDS have landed (and its reads of LDS are done); no access moves across
 __device__ __forceinline__ void lds_landed() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt(0);
@@ -170,7 +170,7 @@ __device__ __forceinline__ void tile_issue(const TileSrc<RT>& t, int k, int H, i
 }
 // all loads of this wavefront into LDS have landed, all its reads are done; then the same holds for the block
 __device__ __forceinline__ void tile_wait() {
-  __builtin_amdgcn_s_waitcnt(0);
+  lds_landed();
   __syncthreads();
 }
 template <int DT, int RT>

@@ -469,19 +469,35 @@ def dense_offsets(M: int, device) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------- adapters
-def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> Permutation:
+class AdapterPlan:
+    """The tokens of a batch sorted by adapter: one buffer with what ``omni_moe_permute`` makes of them."""
+    __slots__ = ("T", "n", "buffer", "sorted_src", "offsets")   # the last two: addresses inside the buffer
+
+
+def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
     """The tokens of a batch sorted by adapter, for ``adapter_linear``: ``adapter_ids`` [T] integers, the adapter of each
     token; a value outside [0, n_adapters) (-1, say) means none.  Made once for a batch and used by all its
     projections."""
-    _need_gpu(adapter_ids)
+    device = _one_device("adapter_plan", adapter_ids)
     if adapter_ids.dim() != 1 or adapter_ids.dtype not in (torch.int32, torch.int64):
         raise ValueError("adapter_plan: adapter_ids must be [T], int32 or int64")
-    if n_adapters < 1:
+    n = int(n_adapters)
+    if n < 1:
         raise ValueError("adapter_plan: at least one adapter")
     if adapter_ids.dtype == torch.int64:  # what int32 cannot hold is no adapter either
-        adapter_ids = torch.where((adapter_ids >= 0) & (adapter_ids < n_adapters), adapter_ids, -1)
-    with torch.cuda.device(adapter_ids.device):
-        return moe_permute(adapter_ids.view(-1, 1), 0, int(n_adapters))
+        adapter_ids = torch.where((adapter_ids >= 0) & (adapter_ids < n), adapter_ids, -1).to(torch.int32)
+    adapter_ids = adapter_ids.contiguous()
+    lib, p = L.lib(), AdapterPlan()
+    p.T, p.n = adapter_ids.shape[0], n
+    ws_bytes = lib.omni_moe_permute_workspace_bytes(p.T, 1, n)
+    # sorted_src [T], src_to_dst [T], counts [n], offsets [n + 1], then the sort's workspace
+    ws_at = (8 * p.T + 8 * n + 4 + 255) // 256 * 256
+    p.buffer = torch.empty((ws_at + ws_bytes,), dtype=torch.uint8, device=adapter_ids.device)
+    at = p.buffer.data_ptr()
+    p.sorted_src, p.offsets = at, at + 8 * p.T + 4 * n
+    _launch(device, "omni_moe_permute", lib.omni_moe_permute, adapter_ids.data_ptr(), p.T, 1, 0, n, L.OMNI_IDX_TOKEN_MAJOR, at,
+            at + 4 * p.T, at + 8 * p.T, p.offsets, at + ws_at, ws_bytes)
+    return p
 
 
 def _vector_rows(t: torch.Tensor, cols: int) -> torch.Tensor:
@@ -505,7 +521,7 @@ def _widths(slices: tuple):
     return arr
 
 
-def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: Permutation,
+def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torch.Tensor, plan: AdapterPlan,
                    scale: Optional[torch.Tensor] = None, slices=None, out: Optional[torch.Tensor] = None,
                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A shared projection's rows with the low-rank update of each token's adapter:
@@ -517,7 +533,7 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     multiples of 8, r at most 256 (shorter ranks are filled up with zeros).  ``out`` may be ``base``.  Both products are
     summed in fp32 and the result is rounded once."""
     what = "adapter_linear"
-    device = _one_device(what, x, base, a, b, scale, plan.sorted_src if plan is not None else None, out, workspace)
+    device = _one_device(what, x, base, a, b, scale, plan.buffer if plan is not None else None, out, workspace)
     _forward_only(what, x, base, a, b, scale, out)
     dt = x.dtype
     if dt not in (torch.bfloat16, torch.float16) or base.dtype != dt or a.dtype != dt or b.dtype != dt:
@@ -539,8 +555,8 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
         raise ValueError(f"{what}: scale must be a contiguous fp32 [{n}] tensor")
     x2, base2 = _vector_rows(x, H), _vector_rows(base, N)
     T = x2.shape[0]
-    if plan.T != T or plan.K != 1 or plan.n_local != n or plan.idx_mode != L.OMNI_IDX_TOKEN_MAJOR:
-        raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n_local} adapters, not {T} and {n}")
+    if plan.T != T or plan.n != n:
+        raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n} adapters, not {T} and {n}")
     if out is None:
         out2 = _like(base2)
         out = out2 if len(bs) == 2 else out2.view(bs)
@@ -561,7 +577,7 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     elif not workspace.is_contiguous():
         raise ValueError(f"{what}: the workspace must be contiguous")
     _launch(device, "omni_adapter_linear", lib.omni_adapter_linear, x2.data_ptr(), _DT[dt], _ld(x2), base2.data_ptr(), _ld(base2),
-            a.data_ptr(), b.data_ptr(), _ptr(scale), plan.sorted_src.data_ptr(), plan.offsets.data_ptr(), T, n, H, r, S,
+            a.data_ptr(), b.data_ptr(), _ptr(scale), plan.sorted_src, plan.offsets, T, n, H, r, S,
             _widths(widths), out2.data_ptr(), _ld(out2), _ptr(workspace), 0 if workspace is None else workspace.nbytes)
     return out
 

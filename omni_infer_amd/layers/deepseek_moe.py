@@ -184,23 +184,24 @@ class DeepseekMoE(nn.Module):
                 next_attention_weights: Optional[dict] = None, adapters=None):
         """``adapters``: an ``AdapterBatch`` of the tokens' low-rank adapters; they act on the shared expert (the routed
         experts have none)."""
-        if self.shared_experts is None or not self.shared_experts.has_adapters:
-            adapters = None
+        # a shared expert of another class knows nothing of adapters, nor need a subclass's body of the forward pass
+        given = () if adapters is None or not getattr(self.shared_experts, "has_adapters", False) else (adapters,)
         opt = model_extra_config.operator_opt_config
         allgather_ep = opt.enable_moe_expert_parallel and self.ep_size > 1 and not (
             opt.prefill_dispatch_combine or opt.moe_dispatch_combine)
         same_width = (self.shared_experts is None or
                       self.shared_experts.down_proj.input_size == self.experts.intermediate_size_per_partition)
         if self.fused and allgather_ep and same_width and self.quant_symbol:
-            return self._forward_fused(hidden_states, attn_metadata, adapters), residual
+            return self._forward_fused(hidden_states, attn_metadata, *given), residual
         if isinstance(hidden_states, dict):
             hidden_states = hidden_states["x"]
-        return self._forward_norm_ops(hidden_states, attn_metadata, adapters), residual
+        return self._forward_norm_ops(hidden_states, attn_metadata, *given), residual
 
     def _forward_norm_ops(self, hidden_states, attn_metadata, adapters=None):
         """deepseek_moe.py:243-305 / :307-368 operator by operator, minus the collectives."""
         opt = model_extra_config.operator_opt_config
-        shared_output = self.shared_experts(hidden_states, adapters) if self.shared_experts is not None else None
+        given = () if adapters is None else (adapters,)
+        shared_output = self.shared_experts(hidden_states, *given) if self.shared_experts is not None else None
         is_prefill = attn_metadata is None or attn_metadata.prefill is not None
         dispatch = opt.prefill_dispatch_combine if is_prefill else opt.moe_dispatch_combine
         if not dispatch and opt.enable_moe_expert_parallel:

@@ -11,6 +11,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -196,12 +197,16 @@ def add_rms_norm_quant(x: torch.Tensor, residual: Optional[torch.Tensor], weight
 # The calls below are short on the GPU (a few microseconds for a decode step), so what they ask of torch is counted:
 # the raw handle of the current stream instead of a Stream object, no views where shapes agree, one pass over the checks.
 def _forward_only(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """The operators have no backward pass: a call that autograd would have to record is refused instead of cutting
-    the graph silently."""
+    """The operators have no derivatives: a call that autograd would have to record is refused instead of cutting the
+    graph silently, and so is one whose inputs carry tangents (which flow under ``torch.no_grad()`` too)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what}: no backward pass is built (call it under torch.no_grad() or detach the inputs)")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}: no forward-mode derivative is built (an input carries a tangent)")
 
 
 def _one_device(what: str, x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> int:

@@ -186,6 +186,7 @@ int omni_swiglu_quant(const void* gate_up, int dtype, int64_t ld, int64_t rows, 
  * an adapter in; ReplicatedLinear / MergedReplicatedLinear, omni/models/common/layers/linear.py:620-762, are where it
  * is added here).
  *   out[t, :] = base[t, :] + (scale[g] * (x[t, :] . A[g]^T)) . B[g]^T for the adapter g of token t, base[t, :] without one
+ *   and where scale[g] is 0 (then whatever x, A and B hold)
  * x [T,H], base and out [T,N] bf16 or fp16 with row strides; A [n, n_slices*r, H], B [n, N, r], scale [n] fp32 or NULL
  * (1).  N is the sum of `widths` (HOST array of n_slices, at most 4): the columns of slice j are multiplied with columns
  * [j*r, (j+1)*r) of x . A^T.  Both products are summed in fp32, the first one is carried with 16 (bf16) or 22 (fp16)

@@ -5,7 +5,8 @@
 // A_g [S*r, H] holds the S slices of a stacked projection (gate and up), B_g [N, r] their output rows one slice under
 // the other; columns of slice j take the columns [j*r, (j+1)*r) of the first product.  The tokens come sorted by
 // adapter (sorted_src and offsets of omni_moe_permute with one assignment per token); tokens without an adapter
-// follow behind the last group and get their base row.
+// follow behind the last group and get their base row, and so do those of an adapter whose scale is zero: by the formula a
+// row or a matrix that is not finite would turn an adapter that adds nothing into NaN, and base's -0 into 0.
 //
 // v = x . A^T is kept in fp32.  The second product wants 16-bit operands on the matrix cores, so v goes in as two of them,
 // hi + lo: 16 bits of mantissa in bf16 (off by at most 2^-16 of it), 22 in fp16, where a row is first brought to a largest
@@ -468,6 +469,10 @@ __device__ __forceinline__ void load_tokens(const AdapterArgs& g, const RowBlock
   if (threadIdx.x < 16 * MS) ((int*)tok)[threadIdx.x] = g.sorted_src[rb.row0 + min((int)threadIdx.x, rb.nrows - 1)];
   __syncthreads();
 }
+// the factor of a group's update; 0: there is none (an adapter of scale 0, or the group without an adapter)
+__device__ __forceinline__ float group_scale(const AdapterArgs& g, int group) {
+  return group >= g.n ? 0.0f : g.scale ? g.scale[group] : 1.0f;
+}
 // which slice and which of its column blocks unit `u` of a launch names; a unit is g.unit_blocks column blocks
 __device__ __forceinline__ Columns find_columns(const AdapterArgs& g, int u, int group, int& slice) {
   slice = 0;
@@ -516,7 +521,8 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
   if (!find_tile(g, none, 16 * MS, (int)blockIdx.x / 8 / g.units * 8 + (int)blockIdx.x % 8, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
-  const bool has = rb.group < g.n;
+  const float sc = group_scale(g, rb.group);
+  const bool has = sc != 0.0f;
   int slice;
   const Columns c = find_columns(g, unit, rb.group, slice);
   const int P = min(g.r, 64) / 8;
@@ -534,7 +540,6 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
   uint16_t* hi = (uint16_t*)(dyn + 4 * WAVE * P);
   uint16_t* lo = hi + 16 * MS * ldk;
   if (has) {
-    const float sc = g.scale ? g.scale[rb.group] : 1.0f;
     const size_t part = (size_t)g.T * g.R;
     const int l = threadIdx.x % 16;  // a row of v by 16 lanes, four values at a time
 #pragma unroll
@@ -598,7 +603,8 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(Adapt
   if (!find_tile(g, none, 16, (int)blockIdx.x / 8 / g.units * 8 + (int)blockIdx.x % 8, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
-  const bool has = rb.group < g.n;
+  const float sc = group_scale(g, rb.group);
+  const bool has = sc != 0.0f;
   int slice;
   const Columns c = find_columns(g, unit, rb.group, slice);
   const int P = g.r / 8;
@@ -613,7 +619,6 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(Adapt
     base_load<1>(o, g, c, blk, tok, m, q);
   }
   if (has) {
-    const float sc = g.scale ? g.scale[rb.group] : 1.0f;
     v4f acc[RT];
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[j] = v4f{0, 0, 0, 0};

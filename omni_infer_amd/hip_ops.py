@@ -534,9 +534,10 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
 
     ``x`` [..., H] went into the projection, ``base`` [..., N] came out of it.  ``a`` [n, S*r, H] and ``b`` [n, N, r] hold n
     adapters; ``slices`` are the S output widths of a stacked projection (gate and up; default: one slice), whose
-    columns take rows j*r..(j+1)*r of ``a``.  ``scale`` [n] fp32 (default 1).  bf16 or fp16; H, r and the widths are
-    multiples of 8, r at most 256 (shorter ranks are filled up with zeros).  ``out`` may be ``base``.  Both products are
-    summed in fp32 and the result is rounded once."""
+    columns take rows j*r..(j+1)*r of ``a``.  ``scale`` [n] fp32 (default 1; an adapter of scale 0 adds nothing, whatever
+    the rows and its matrices hold).  bf16 or fp16; H, r and the widths are multiples of 8, r at most 256 (shorter ranks
+    are filled up with zeros).  ``out`` may be ``base``.  Both products are summed in fp32 and the result is rounded
+    once."""
     what = "adapter_linear"
     device = _one_device(what, x, base, a, b, scale, plan.buffer if plan is not None else None, out, workspace)
     _forward_only(what, x, base, a, b, scale, out)

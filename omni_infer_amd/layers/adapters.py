@@ -30,8 +30,9 @@ class AdapterBatch:
 
 class AdapterSlots(nn.Module):
     """The adapters of one projection with the output widths ``output_sizes`` (one, or the shards of a stacked one).
-    A slot that holds nothing adds nothing; shorter ranks are filled up with zeros to ``max_rank``, which is rounded
-    up to a multiple of 8."""
+    A slot that holds nothing has the scale 0, which adds nothing whatever the rows hold.  Shorter ranks and shards that an
+    adapter leaves alone are filled up with zeros to ``max_rank``, which is rounded up to a multiple of 8: a row of x that
+    is not finite comes out as NaN there, where infinities times those zeros meet."""
 
     def __init__(self, input_size: int, output_sizes: Sequence[int], max_adapters: int, max_rank: int,
                  dtype: torch.dtype = torch.bfloat16, device=None):

@@ -476,13 +476,39 @@ def dense_offsets(M: int, device) -> torch.Tensor:
 # ----------------------------------------------------------------------------- adapters
 class AdapterPlan:
     """The tokens of a batch sorted by adapter: one buffer with what ``omni_moe_permute`` makes of them."""
-    __slots__ = ("T", "n", "buffer", "sorted_src", "offsets")   # the last two: addresses inside the buffer
+    __slots__ = ("T", "n", "buffer", "sorted_src", "offsets",   # the last two: addresses inside the buffer
+                 "stream", "joined")   # the stream it was made on (None inside a capture), streams that are behind the sort
+
+
+def _capturing(device: int) -> bool:
+    if device == torch._C._cuda_getDevice():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _join_plan(plan: AdapterPlan, device: int) -> None:
+    """Lets the current stream use a plan that was made on another one: what the kernels read from it are places in
+    memory, so neither a sort that has not run yet nor memory that was given to someone else may be read.  A stream being
+    captured cannot wait for work outside; the capture's own start lies behind the plan."""
+    raw = torch._C._cuda_getCurrentRawStream(device)
+    if raw in plan.joined:
+        return
+    stream = torch.cuda.current_stream(device)
+    if plan.stream is None:
+        plan.joined.add(raw)
+    elif not _capturing(device):
+        stream.wait_stream(plan.stream)
+        plan.joined.add(raw)
+    plan.buffer.record_stream(stream)
 
 
 def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
     """The tokens of a batch sorted by adapter, for ``adapter_linear``: ``adapter_ids`` [T] integers, the adapter of each
     token; a value outside [0, n_adapters) (-1, say) means none.  Made once for a batch and used by all its
-    projections."""
+    projections, also on other streams: the first use there waits for what the plan's stream has been given so far.  A
+    graph that uses a plan made outside of it reads the plan's memory at every replay, so the plan has to live as long
+    as the graph; one made inside is made anew by every replay and means nothing before the first."""
     device = _one_device("adapter_plan", adapter_ids)
     if adapter_ids.dim() != 1 or adapter_ids.dtype not in (torch.int32, torch.int64):
         raise ValueError("adapter_plan: adapter_ids must be [T], int32 or int64")
@@ -502,6 +528,8 @@ def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
     p.sorted_src, p.offsets = at, at + 8 * p.T + 4 * n
     _launch(device, "omni_moe_permute", lib.omni_moe_permute, adapter_ids.data_ptr(), p.T, 1, 0, n, L.OMNI_IDX_TOKEN_MAJOR, at,
             at + 4 * p.T, at + 8 * p.T, p.offsets, at + ws_at, ws_bytes)
+    p.joined = {torch._C._cuda_getCurrentRawStream(device)}
+    p.stream = None if _capturing(device) else torch.cuda.current_stream(device)
     return p
 
 
@@ -563,6 +591,7 @@ def adapter_linear(x: torch.Tensor, base: torch.Tensor, a: torch.Tensor, b: torc
     T = x2.shape[0]
     if plan.T != T or plan.n != n:
         raise ValueError(f"{what}: the plan is for {plan.T} tokens and {plan.n} adapters, not {T} and {n}")
+    _join_plan(plan, device)
     if out is None:
         out2 = _like(base2)
         out = out2 if len(bs) == 2 else out2.view(bs)

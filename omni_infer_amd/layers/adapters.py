@@ -21,7 +21,8 @@ from .. import hip_ops as ops
 
 
 class AdapterBatch:
-    """Which adapter each token of a batch uses, sorted once for all projections of all layers."""
+    """Which adapter each token of a batch uses, sorted once for all projections of all layers, on whatever streams they
+    run (``hip_ops.adapter_plan`` for what holds under graph capture)."""
 
     def __init__(self, adapter_ids: torch.Tensor, max_adapters: int):
         self.max_adapters = int(max_adapters)

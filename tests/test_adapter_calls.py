@@ -50,3 +50,91 @@ def test_a_slot_that_holds_nothing(T):
     got = slots.add_to(base.clone(), x.cuda(), AdapterBatch(ids.cuda(), 3))
     held = ids.cuda() == 0
     assert torch.equal(got[~held], base[~held]) and not torch.equal(got[held], base[held])
+
+
+# ------------------------------------------------------------------ a plan on another stream than its own
+class _Recorded:
+    def __init__(self):
+        self.log = []
+
+    def record_stream(self, s):
+        self.log.append(("record", s.cuda_stream))
+
+
+class _FakeStream:
+    def __init__(self, handle, log):
+        self.cuda_stream, self.log = handle, log
+
+    def wait_stream(self, s):
+        self.log.append(("wait", s))
+
+
+@pytest.mark.parametrize("capturing", [False, True])
+def test_a_plan_joins_the_stream_that_uses_it(capturing, monkeypatch):
+    """The first use of a plan on another stream waits until the plan is made and holds its memory for that stream; a stream being
+    captured cannot wait for what happened outside."""
+    from omni_infer_amd import hip_ops as ops
+    plan, buf = ops.AdapterPlan(), _Recorded()
+    plan.buffer, plan.stream, plan.joined = buf, "its stream", {7}
+    monkeypatch.setattr(ops, "_capturing", lambda device: capturing)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: _FakeStream(9, buf.log))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 7, raising=False)
+    ops._join_plan(plan, 0)
+    assert buf.log == []                      # its own stream
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 9, raising=False)
+    ops._join_plan(plan, 0)
+    want = [("record", 9)] if capturing else [("wait", "its stream"), ("record", 9)]
+    assert buf.log == want
+    ops._join_plan(plan, 0)
+    assert buf.log == (want * 2 if capturing else want)      # once for a stream
+    plan.stream, plan.joined = None, {7}                       # made inside a capture: its streams are joined by whoever captures
+    del buf.log[:]
+    ops._join_plan(plan, 0)
+    assert buf.log == [("record", 9)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n,r,H,widths", FORMS)
+def test_a_plan_made_on_one_stream_and_used_on_another(T, n, r, H, widths):
+    """Without a word about streams from the caller: the plan lies behind long work of its stream, and its memory is given away
+    while the other stream still has work to do with it."""
+    from omni_infer_amd import hip_ops as ops
+    d = make(T, n, r, H, widths, BF16, seed=T)
+    want = run(d)
+    m = torch.randn(4096, 4096, device="cuda").to(BF16)
+    out = torch.empty_like(m)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            for _ in range(20):
+                torch.mm(m, m, out=out)
+            plan = ops.adapter_plan(d["ids"], n)
+        with torch.cuda.stream(s2):
+            got = ops.adapter_linear(d["x"], d["base"], d["a"], d["b"], plan, d["scale"], slices=d["widths"])
+        size = plan.buffer.numel()
+        del plan
+        with torch.cuda.stream(s1):
+            waste = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del waste
+
+
+@pytest.mark.gpu
+def test_a_plan_made_before_a_capture_is_used_in_it():
+    from omni_infer_amd import hip_ops as ops
+    for T, n, r, H, widths in FORMS:
+        d = make(T, n, r, H, widths, BF16, seed=T)
+        plan = ops.adapter_plan(d["ids"], n)
+        call = lambda: ops.adapter_linear(d["x"], d["base"], d["a"], d["b"], plan, d["scale"], slices=d["widths"])  # noqa: E731
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = call()
+        for k in range(3):
+            d["x"].copy_(torch.randn(T, H, device="cuda"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, call())

@@ -86,14 +86,18 @@ def lib() -> ctypes.CDLL:
         # devices: make sure torch is loaded first.
         import torch  # noqa: F401
         handle = ctypes.CDLL(LIB_PATH)
+        rebuild = "rebuild it with `python -m omni_infer_amd._build`"
+        # the number goes up when an entry changes; entries that are new show by their names
+        version = getattr(handle, "omni_moe_abi_version", None)
+        have = version() if version is not None else None
+        if have != ABI_VERSION:
+            raise OmniMoeError(f"{LIB_PATH} has ABI version {have}, this package binds version {ABI_VERSION}: {rebuild}")
         for name, (res, args) in SIGNATURES.items():
-            fn = getattr(handle, name)  # AttributeError if the library does not export it
+            fn = getattr(handle, name, None)
+            if fn is None:
+                raise OmniMoeError(f"{LIB_PATH} has no {name}: {rebuild}")
             fn.restype = res
             fn.argtypes = args
-        have = handle.omni_moe_abi_version()
-        if have != ABI_VERSION:
-            raise OmniMoeError(f"{LIB_PATH} has ABI version {have}, this package binds version {ABI_VERSION}: "
-                               "rebuild it with `python -m omni_infer_amd._build`")
         _lib = handle
     return _lib
 

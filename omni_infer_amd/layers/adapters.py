@@ -69,13 +69,15 @@ class AdapterSlots(nn.Module):
                                   tuple(b.shape) != (width, a.shape[0]) or a.shape[0] > self.rank):
                 raise ValueError(f"set_adapter: [rank, {self.a.shape[2]}] and [{width}, rank] with a rank up to "
                                  f"{self.rank}, not {tuple(a.shape)} and {tuple(b.shape)}")
-        self.clear(slot)
+        new_a, new_b = torch.zeros_like(self.a.data[slot]), torch.zeros_like(self.b.data[slot])
         for j, (a, b, width) in enumerate(zip(lora_a, lora_b, self.output_sizes)):
             if a is not None:
                 k = a.shape[0]
-                self.a.data[slot, j * self.rank:j * self.rank + k].copy_(a)
-                self.b.data[slot, n0:n0 + width, :k].copy_(b)
+                new_a[j * self.rank:j * self.rank + k].copy_(a)
+                new_b[n0:n0 + width, :k].copy_(b)
             n0 += width
+        self.a.data[slot].copy_(new_a)   # all at once: what was given may lie in this slot
+        self.b.data[slot].copy_(new_b)
         self.scale.data[slot] = float(scaling)
 
     def clear(self, slot: int) -> None:

@@ -138,3 +138,21 @@ def test_a_plan_made_before_a_capture_is_used_in_it():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, call())
+
+
+# ------------------------------------------------------------------ slots filled from slots
+def test_a_slot_is_set_from_its_own_matrices():
+    """To change its scale, to take off its last ranks, to move it to the other shard."""
+    from omni_infer_amd.layers.adapters import AdapterSlots
+    s = AdapterSlots(24, [16, 16], 2, 8)
+    a, b = torch.randn(6, 24).to(BF16), torch.randn(16, 6).to(BF16)
+    s.set_adapter(1, [a, None], [b, None], 0.5)
+    s.set_adapter(1, [s.a.data[1, :6], None], [s.b.data[1, :16, :6], None], 0.25)
+    assert torch.equal(s.a[1, :6], a) and torch.equal(s.b[1, :16, :6], b) and float(s.scale[1]) == 0.25
+    s.set_adapter(1, [s.a.data[1, 2:6], None], [s.b.data[1, :16, 2:6], None])
+    assert torch.equal(s.a[1, :4], a[2:]) and torch.equal(s.b[1, :16, :4], b[:, 2:]) and not bool(s.a[1, 4:].any())
+    s.set_adapter(1, [None, s.a.data[1, :4]], [None, s.b.data[1, :16, :4]])
+    assert torch.equal(s.a[1, 8:12], a[2:]) and torch.equal(s.b[1, 16:, :4], b[:, 2:])
+    assert not bool(s.a[1, :8].any()) and not bool(s.b[1, :16].any()) and not bool(s.a[1, 12:].any()) and not bool(s.b[1, :, 4:].any())
+    s.set_adapter(0, [s.a.data[1, 8:12]] * 2, [s.b.data[1, 16:, :4]] * 2)
+    assert torch.equal(s.a[0, :4], a[2:]) and torch.equal(s.a[0, 8:12], a[2:]) and torch.equal(s.b[0, 16:, :4], b[:, 2:])

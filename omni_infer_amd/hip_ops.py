@@ -266,8 +266,9 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     end_b = pb + ((b.shape[0] - 1) * _ld(b) + b.shape[1]) * eb
     if end_a <= pb or end_b <= pa:
         return False
-    pitch = _ld(a) * ea
-    if pitch == _ld(b) * eb and a.shape[0] > 1 and b.shape[0] > 1:
+    pitches = {_ld(t) * e for t, e in ((a, ea), (b, eb)) if t.shape[0] > 1}   # a single row has none
+    if len(pitches) == 1:
+        pitch = pitches.pop()
         at = (pb - pa) % pitch
         return not (at >= a.shape[1] * ea and at + b.shape[1] * eb <= pitch)
     return True
@@ -314,12 +315,16 @@ def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Te
             mode, ldg = L.OMNI_GATE_TOKEN, _ld(g2)
         else:
             raise ValueError(f"{what}: the gate must be [{H}], [..., 1] or of x's shape")
+    if not (post_weight.is_contiguous() and pre_weight.is_contiguous()):
+        post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
     if inplace_residual:
         if r2.data_ptr() != residual.data_ptr():
             raise ValueError(f"{what}: a residual with these strides cannot be written in place")
         out, res_out = r2, residual
         same = x2.data_ptr() == r2.data_ptr() and _ld(x2) == _ld(r2)
-        if (not same and _overlap(x2, out)) or (mode in (L.OMNI_GATE_TOKEN, L.OMNI_GATE_FULL) and _overlap(g2, out)):
+        # rows are worked on in no order: one may read what another has written
+        if (not same and _overlap(x2, out)) or (g2 is not None and _overlap(g2 if g2.dim() == 2 else g2.view(1, -1), out)) or (
+                _overlap(post_weight.view(1, -1), out) or _overlap(pre_weight.view(1, -1), out)):
             raise ValueError(f"{what}: the residual written in place overlaps another input")
     else:
         out = _like(x2)
@@ -329,8 +334,6 @@ def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Te
     if want_quant:
         q = _like(x2, torch.int8)
         sc = torch.empty((rows,), dtype=torch.float32, device=x.device)
-    if not (post_weight.is_contiguous() and pre_weight.is_contiguous()):
-        post_weight, pre_weight = post_weight.contiguous(), pre_weight.contiguous()
     _launch(device, "omni_sandwich_norm", L.lib().omni_sandwich_norm, x2.data_ptr(), _DT[dt], _ld(x2), r2.data_ptr(), _ld(r2),
             post_weight.data_ptr(), pre_weight.data_ptr(), _ptr(g2), mode, ldg, rows, H, post_eps, pre_eps, residual_scale,
             out.data_ptr(), _ld(out), _ptr(y), _ptr(q), _ptr(sc))

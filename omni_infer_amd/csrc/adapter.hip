@@ -695,14 +695,15 @@ int launch_adapter(AdapterArgs& g, const omni_host::AdapterPlan& p, hipStream_t 
   const int kp = g.r <= 16 ? 16 : (g.r + 31) / 32 * 32;
   const size_t shm = (size_t)4 * WAVE * (g.r < 64 ? g.r / 8 : 8) * 16 + (size_t)2 * 16 * p.out_row_tiles * (kp + 8) * 2;
   const dim3 grid2((unsigned)((p.out_tiles_max + (g.in_place ? 0 : 1) + 7) / 8 * 8 * g.units));
-#define EXPAND(MS)                                                                                                   \
-  do {                                                                                                           \
-    if (g.r <= 32) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 4>), grid2, dim3(256), shm, st, g);      \
-    else if (g.r <= 64) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 1, 8>), grid2, dim3(256), shm, st, g); \
-    else hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, 4, 8>), grid2, dim3(256), shm, st, g);                \
-  } while (0)
-  if (p.out_row_tiles == 1) EXPAND(1);
-  else EXPAND(2);
+#define EXPAND(MS, KQ, PMAX) hipLaunchKernelGGL((adapter_expand_kernel<DT, MS, KQ, PMAX>), grid2, dim3(256), shm, st, g)
+  if (p.out_row_tiles == 2) {  // ranks of 33 to 128
+    if (g.r <= 64) EXPAND(2, 1, 8);
+    else EXPAND(2, 4, 8);
+  } else {
+    if (g.r <= 32) EXPAND(1, 1, 4);
+    else if (g.r <= 64) EXPAND(1, 1, 8);
+    else EXPAND(1, 4, 8);
+  }
 #undef EXPAND
   OMNI_CHECK_LAUNCH("adapter_linear");
   return OMNI_OK;

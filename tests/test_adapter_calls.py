@@ -1,9 +1,14 @@
 """Calls of the adapters beside the tests of their formula: slots that hold nothing, batches on other streams, every kernel the
 dispatch can choose."""
+import os
+import re
+import shutil
+import subprocess
+
 import pytest
 import torch
 
-from tests.test_adapter import BF16, FP16, check, make, run
+from tests.test_adapter import BF16, FP16, ROOT, check, make, run
 
 # tokens, adapters, rank, H, widths: one launch; two launches with 16-row blocks; with 128-row blocks
 FORMS = [(20, 4, 24, 136, [72]), (65, 3, 128, 264, [136, 64]), (1200, 4, 40, 264, [72, 128])]
@@ -156,3 +161,71 @@ def test_a_slot_is_set_from_its_own_matrices():
     assert not bool(s.a[1, :8].any()) and not bool(s.b[1, :16].any()) and not bool(s.a[1, 12:].any()) and not bool(s.b[1, :, 4:].any())
     s.set_adapter(0, [s.a.data[1, 8:12]] * 2, [s.b.data[1, 16:, :4]] * 2)
     assert torch.equal(s.a[0, :4], a[2:]) and torch.equal(s.a[0, 8:12], a[2:]) and torch.equal(s.b[0, 16:, :4], b[:, 2:])
+
+
+# ------------------------------------------------------------------ every kernel the dispatch can choose
+# What one launch does not take: prompts of many adapters, ranks above 16 at wide H, ranks above 64; odd numbers of tokens
+# and widths that fill no tile; sums in one part and in many; more adapters than a wavefront has lanes
+DISPATCH = [  # T, n, r, H, widths
+    (1024, 64, 16, 4096, [4096]),
+    (1024, 64, 16, 4096, [2048, 2048]),
+    (64, 32, 64, 4096, [4096]),
+    (64, 32, 16, 16384, [5120]),
+    (512, 256, 16, 7168, [2048, 2048]),
+    (1, 4, 32, 7168, [2048, 2048]),
+    (1, 4, 64, 7168, [2048, 2048]),
+    (1031, 66, 8, 4104, [1048]),
+    (1025, 100, 16, 1992, [200, 72]),
+    (2040, 256, 32, 520, [72]),
+    (77, 9, 56, 5000, [136, 1032]),
+    (3, 2, 40, 7176, [264]),
+    (1100, 64, 64, 328, [72]),
+    (1040, 100, 32, 520, [40, 72, 24]),
+    (65, 3, 128, 264, [136, 64]),
+    (130, 3, 256, 136, [264]),
+    (1200, 5, 16, 136, [72]),
+    (1200, 5, 40, 264, [200]),
+    (1111, 3, 24, 1992, [40, 72, 24]),
+    (1025, 3, 64, 4104, [128, 24]),
+    (1030, 1, 72, 4104, [64, 72]),
+    (1300, 2, 256, 328, [200]),
+    (1, 4, 16, 7168, [2048, 2048]),
+    (333, 12, 24, 1992, [1048]),
+    (33, 2, 56, 136, [200]),
+]
+
+
+def _chosen(tmp_path, cases):
+    exe = str(tmp_path / "adapter_dispatch")
+    subprocess.run([shutil.which("g++"), "-std=c++17", "-O1", os.path.join(ROOT, "tests", "host", "adapter_dispatch.cpp"), "-o", exe], check=True)
+    lines = "".join(f"{T} {n} {H} {r} {len(w)} {sum(w)}\n" for T, n, r, H, w in cases)
+    at = subprocess.run([exe, "-"], input=lines, capture_output=True, text=True, check=True, timeout=60).stdout.splitlines()
+    every = subprocess.run([exe], capture_output=True, text=True, check=True, timeout=60).stdout.splitlines()
+    return [tuple(a.split(" parts ")) for a in at], set(every)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not available")
+def test_the_cases_reach_every_kernel_of_the_dispatch(tmp_path):
+    """A rule that is changed later must not leave a kernel without a case; and no kernel is there that no shape reaches."""
+    at, every = _chosen(tmp_path, DISPATCH)
+    assert {k for k, _ in at} == every
+    assert {int(parts) for _, parts in at} >= {1, 3, 8, 14}
+    text = open(os.path.join(ROOT, "omni_infer_amd", "csrc", "adapter.hip")).read()
+    seconds = {k.split()[1] for k in every if " " in k}
+    assert seconds == {"out1_32", "out1_64", "out1_256", "out2_64", "out2_256"}
+    assert len(set(re.findall(r"EXPAND\((\d), (\d), (\d)\);", text))) == len(seconds)
+    assert {k.split()[0] for k in every} == {"one_launch_16", "one_launch_32", "one_launch_64", "rows_16", "rows_32", "rows_64",
+                                             "rows_128", "tile_64", "tile_128"}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,n,r,H,widths", DISPATCH)
+def test_every_kernel_against_the_formula(T, n, r, H, widths, dtype):
+    d = make(T, n, r, H, widths, dtype, seed=T + r + n)
+    got = run(d)
+    check(got, d)
+    assert torch.equal(got, run(d)), "two calls differ"
+    out = d["base"].clone()
+    assert run(dict(d, base=out), out=out) is out
+    assert torch.equal(out, got), "in place"

@@ -229,3 +229,53 @@ def test_every_kernel_against_the_formula(T, n, r, H, widths, dtype):
     out = d["base"].clone()
     assert run(dict(d, base=out), out=out) is out
     assert torch.equal(out, got), "in place"
+
+
+# ------------------------------------------------------------------ two calls at once, each with partial sums in memory
+@pytest.mark.gpu
+def test_two_streams_with_workspaces():
+    """Two launches with sums of their own between them (workspaces of different sizes, some in many parts), one launch beside."""
+    from omni_infer_amd import _lib as L
+    shapes = [(1200, 5, 16, 2048, [512]), (1100, 3, 128, 1024, [768]), (40, 6, 64, 7168, [1024, 1024]), (700, 5, 16, 2048, [512])]
+    need = [L.lib().omni_adapter_linear_workspace_bytes(T, n, H, r, len(w), sum(w)) for T, n, r, H, w in shapes]
+    assert len(set(need[:3])) == 3 and min(need[:3]) > 0 and need[3] == 0
+    ds = [make(*s, BF16, seed=k) for k, s in enumerate(shapes)]
+    want = [run(d) for d in ds]
+    for d, w in zip(ds, want):
+        check(w, d)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for k in range(12):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                i = (k + j) % len(ds) if k < 8 else k % len(ds)     # different ones beside each other, then twice the same
+                got.append((i, run(ds[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i, g in got)
+
+
+@pytest.mark.gpu
+def test_two_graphs_with_workspaces():
+    """Recorded and replayed beside each other on two streams: a graph's partial sums are its own."""
+    shapes = [(1200, 5, 16, 2048, [512]), (40, 6, 64, 7168, [1024, 1024])]
+    made = []
+    for k, s in enumerate(shapes):
+        d = make(*s, BF16, seed=k)
+        run(d)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(d)
+        made.append((d, graph, got))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for k in range(4):
+        for d, _, _ in made:
+            d["x"].copy_(torch.randn(d["x"].shape, generator=torch.Generator().manual_seed(k)))
+        torch.cuda.synchronize()
+        for s, (_, graph, _) in zip(streams, made):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for d, _, got in made:
+            assert torch.equal(got, run(d)), k

@@ -131,9 +131,14 @@ def _own(s, case):
         y, residual, q, scale = hip_ops.sandwich_norm(
             s["x"], s["residual"], s["post_weight"], s["pre_weight"], POST_EPS, PRE_EPS, gate=s["gate"],
             residual_scale=RESIDUAL_SCALE, want_y=not quant, want_quant=quant)
-        return (torch.mul(q, scale.unsqueeze(-1), out=s["values"]) if quant else y), residual
+        return (_values(q, scale, s) if quant else y), residual
     h, q, scale = hip_ops.swiglu_quant(s["gate_up"], want_quant=quant)
-    return (h, torch.mul(q, scale.unsqueeze(-1), out=s["values"])) if quant else h
+    return (h, _values(q, scale, s)) if quant else h
+
+
+def _values(q, scale, s):
+    """What int8 rows stand for, in a tensor of each pass's own, as the plain form gives them."""
+    return torch.mul(q, scale.unsqueeze(-1), out=torch.empty_like(s["values"]))
 
 
 def _adapter(s, case):

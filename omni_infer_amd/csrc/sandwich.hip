@@ -60,10 +60,17 @@ __global__ __launch_bounds__(THREADS) void sandwich_norm_kernel(SandwichArgs a) 
       load8<DT, ALIGNED>((const ET*)a.post_w, vi, H, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[i][j] = (s[i][j] * r1) * w[j];
-      if (wide_gate) load8<DT, ALIGNED>(gr, vi, H, w);
+      if (wide_gate) {
+        load8<DT, ALIGNED>(gr, vi, H, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i][j] = (a.c * w[j]) * s[i][j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[i][j] = c * s[i][j];
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        s[i][j] = d[i][j] + (wide_gate ? a.c * w[j] : c) * s[i][j];
+        s[i][j] = d[i][j] + s[i][j];
         ss = ss + (vi * 8 + j < H ? s[i][j] * s[i][j] : 0.0f);
       }
       store8<DT, ALIGNED>((ET*)a.residual_out + r * a.ldo, vi, H, s[i]);

@@ -366,8 +366,8 @@ __device__ __forceinline__ void base_load(ExpandOps<MS>& o, const AdapterArgs& g
 // one column block whose panel (the first 64 of the rank) and base values are here or on their way
 template <int DT, int MS, int PMAX>
 __device__ __forceinline__ void expand_block(const ExpandOps<MS>& o, const Panel<PMAX>& pn, int P, v4i* panel, const AdapterArgs& g,
-                                             const Columns& c, int blk, const RowBlock& rb, bool has, const v4i* tok, int m, int q,
-                                             const uint16_t* hi, const uint16_t* lo, int ldk, const float* unscale) {
+                                             const Columns& c, int blk, const RowBlock& rb, bool has, float sc, const v4i* tok,
+                                             int m, int q, const uint16_t* hi, const uint16_t* lo, int ldk, const float* unscale) {
   v4f acc[MS][4];
 #pragma unroll
   for (int i = 0; i < MS; ++i)
@@ -431,7 +431,7 @@ __device__ __forceinline__ void expand_block(const ExpandOps<MS>& o, const Panel
       const int row = i * 16 + q * 4 + e;
       if (row >= rb.nrows || col >= c.width) continue;
       v2i v = o.base[i][e];
-      if (has) {
+      if (sc != 0.0f) {
         float un = 1.0f;
         if constexpr (DT == OMNI_DT_F16) un = unscale[row];
 #pragma unroll
@@ -450,7 +450,7 @@ __device__ __forceinline__ void expand_block(const ExpandOps<MS>& o, const Panel
 // The column blocks of one wavefront.  The first block's panel and base values are on their way when `o` and `blk` come in.
 template <int DT, int MS, int PMAX>
 __device__ __forceinline__ void expand_columns(ExpandOps<MS>& o, const Panel<PMAX>& pn, int P, v4i* panel, const AdapterArgs& g,
-                                               const Columns& c, int blk, int step, const RowBlock& rb, bool has, const v4i* tok,
+                                               const Columns& c, int blk, int step, const RowBlock& rb, bool has, float sc, const v4i* tok,
                                                int m, int q, const uint16_t* hi, const uint16_t* lo, int ldk, const float* unscale) {
   for (bool first = true; blk < c.blk_end; blk += step, first = false) {
     if (!first) {
@@ -460,7 +460,7 @@ __device__ __forceinline__ void expand_columns(ExpandOps<MS>& o, const Panel<PMA
       }
       base_load<MS>(o, g, c, blk, tok, m, q);
     }
-    expand_block<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, rb, has, tok, m, q, hi, lo, ldk, unscale);
+    expand_block<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, rb, has, sc, tok, m, q, hi, lo, ldk, unscale);
   }
 }
 // the tokens of a block's rows; rows past the last repeat it
@@ -468,10 +468,6 @@ template <int MS>
 __device__ __forceinline__ void load_tokens(const AdapterArgs& g, const RowBlock& rb, v4i* tok) {
   if (threadIdx.x < 16 * MS) ((int*)tok)[threadIdx.x] = g.sorted_src[rb.row0 + min((int)threadIdx.x, rb.nrows - 1)];
   __syncthreads();
-}
-// the factor of a group's update; 0: there is none (an adapter of scale 0, or the group without an adapter)
-__device__ __forceinline__ float group_scale(const AdapterArgs& g, int group) {
-  return group >= g.n ? 0.0f : g.scale ? g.scale[group] : 1.0f;
 }
 // which slice and which of its column blocks unit `u` of a launch names; a unit is g.unit_blocks column blocks
 __device__ __forceinline__ Columns find_columns(const AdapterArgs& g, int u, int group, int& slice) {
@@ -521,8 +517,8 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
   if (!find_tile(g, none, 16 * MS, (int)blockIdx.x / 8 / g.units * 8 + (int)blockIdx.x % 8, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
-  const float sc = group_scale(g, rb.group);
-  const bool has = sc != 0.0f;
+  const bool has = rb.group < g.n;
+  float sc = 0.0f;  // of a group without an adapter, too: nothing is added
   int slice;
   const Columns c = find_columns(g, unit, rb.group, slice);
   const int P = min(g.r, 64) / 8;
@@ -540,6 +536,7 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
   uint16_t* hi = (uint16_t*)(dyn + 4 * WAVE * P);
   uint16_t* lo = hi + 16 * MS * ldk;
   if (has) {
+    sc = g.scale ? g.scale[rb.group] : 1.0f;
     const size_t part = (size_t)g.T * g.R;
     const int l = threadIdx.x % 16;  // a row of v by 16 lanes, four values at a time
 #pragma unroll
@@ -575,7 +572,7 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
     }
     __syncthreads();
   }
-  expand_columns<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, 4, rb, has, tok, m, q, hi, lo, ldk, unscale);
+  expand_columns<DT, MS, PMAX>(o, pn, P, panel, g, c, blk, 4, rb, has, sc, tok, m, q, hi, lo, ldk, unscale);
 }
 
 // ---------------------------------------------------------------- both products in one launch
@@ -603,8 +600,8 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(Adapt
   if (!find_tile(g, none, 16, (int)blockIdx.x / 8 / g.units * 8 + (int)blockIdx.x % 8, rb)) return;
   const int lane = threadIdx.x & (WAVE - 1), w = threadIdx.x / WAVE;
   const int m = lane & 15, q = lane >> 4;
-  const float sc = group_scale(g, rb.group);
-  const bool has = sc != 0.0f;
+  const bool has = rb.group < g.n;
+  float sc = 0.0f;  // of a group without an adapter, too: nothing is added
   int slice;
   const Columns c = find_columns(g, unit, rb.group, slice);
   const int P = g.r / 8;
@@ -619,6 +616,7 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(Adapt
     base_load<1>(o, g, c, blk, tok, m, q);
   }
   if (has) {
+    sc = g.scale ? g.scale[rb.group] : 1.0f;
     v4f acc[RT];
 #pragma unroll
     for (int j = 0; j < RT; ++j) acc[j] = v4f{0, 0, 0, 0};
@@ -656,7 +654,7 @@ __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(Adapt
     }
     __syncthreads();
   }
-  expand_columns<DT, 1, PMAX>(o, pn, P, panel, g, c, blk, FUSED_WAVES, rb, has, tok, m, q, lds, lds + 16 * LDK, LDK, unscale);
+  expand_columns<DT, 1, PMAX>(o, pn, P, panel, g, c, blk, FUSED_WAVES, rb, has, sc, tok, m, q, lds, lds + 16 * LDK, LDK, unscale);
 }
 
 int column_units(const AdapterArgs& g, int unit_blocks) {

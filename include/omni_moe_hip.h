@@ -194,6 +194,8 @@ int omni_swiglu_quant(const void* gate_up, int dtype, int64_t ld, int64_t rows, 
  * its last bits may depend on T and n, which choose how the first sum is cut.
  *   sorted_src, offsets: of omni_moe_permute(ids, T, K = 1, lo = 0, hi = n, OMNI_IDX_TOKEN_MAJOR).  Ids outside [0, n):
  *   no adapter.
+ *   A and B are finite: where an infinity stands in B, NaN may come out for it (the first product goes in as two numbers, and
+ *   the second may be zero).  Infinities and NaN in x stay in their rows.
  *   H, r, every width, ldx, ld_base, ld_out multiples of 8, pointers 16-byte aligned; r <= 256, n <= 256, H and N <= 2^20.
  *   out may be base (same stride): rows without an adapter are then left alone.  No other overlap.
  *   workspace: omni_adapter_linear_workspace_bytes(T, n, H, r, n_slices, N), 16-byte aligned; written and read by this

@@ -152,10 +152,11 @@ __device__ __forceinline__ void shrink_chunks(Stage<RT, D>& st, const AdapterArg
 }
 
 // v = x . A^T for many rows: 128 sorted rows of one adapter by 16*RT of its rows and one part of the reduction.  What bounds
-// it is what a compute unit can draw from behind its cache (27 to 30 GB/s), and A counts there like x, so the eight
-// wavefronts share A: chunks of 64 elements go into two stages in turn, two blocks on a compute unit.  Wavefronts lie 4 (32
-// rows each) x 2 (half of the A rows each).  8192 x 7168 tokens by 128 rows of A in 35 to 41 us (117 MB of x, 3 TB/s), where
-// 64 rows a block with operands straight from memory took 72; 8192 x 2048 by 16 rows in 12 us.
+// it is what a compute unit can draw from behind its cache, 27 to 30 GB/s whether the L2 has it or not, and A counts there
+// like x, so the eight wavefronts share A: chunks of 64 elements go into two stages in turn, two blocks on a compute unit.
+// Wavefronts lie 4 (32 rows each) x 2 (half of the A rows each).  8192 x 7168 tokens by 128 rows of A in 35 to 41 us (117 MB
+// of x, 3 TB/s), where 64 rows a block with operands straight from memory took 72: the L2 counts 287 MB of requests, 128 MB of
+// them hits (A), 27 GB/s for each of 256 compute units.  8192 x 2048 by 16 rows in 12 us.
 constexpr int ST_ROWS = 128, ST_WAVES = 8;
 template <int RT>
 struct TileSrc {
@@ -255,7 +256,9 @@ __global__ __launch_bounds__(ST_WAVES * WAVE, 4) void adapter_shrink_tile_kernel
 }
 
 // v = x . A^T for few rows.  A block of four wavefronts takes 16 sorted rows of one adapter, 16*RT of its rows and one part of
-// the reduction, of which every wavefront has its share.
+// the reduction, of which every wavefront has its share.  A single token waits for memory (rank 32 and 64, 7168 -> 2 x 2048:
+// 3.2 and 5.3 us in 14 parts, with 5.3 and 6.0 us for the second product); an adapter per token is bound by A: 64 tokens, about 56
+// adapters in use, rank 32 and 64: 51 and 103 MB in 11 and 22 us, 4.6 TB/s.
 template <int DT, int RT>
 __global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterArgs g) {
   constexpr int D = shrink_depth(RT);
@@ -502,9 +505,9 @@ __device__ __forceinline__ v4f sum_parts(const float* p, size_t step, int n) {
 }
 // out = base + v . B^T from the sums of the first launch.  A block of four wavefronts takes 16*MS sorted rows and a
 // unit of column blocks; a wavefront takes 64 columns at a time.  Bound by base and out, which a plain copy moves in 26 us for
-// 8192 rows of 2 x 2048 and in 45 to 49 us for 8192 of 7168: 51 us at rank 64 (MS = 2; B, read by every block from the L2, is
-// as much again) and 55 us at rank 16 (MS = 1: more wavefronts; MS = 2 takes 61).  16 column blocks a unit: 32
-// take 56 and 62 us.
+// 8192 rows of 2 x 2048 and in 45 to 49 us for 8192 of 7168: 51 us at rank 64 (MS = 2; B and the parts of v, read by every
+// block, are more again: 379 MB of requests to the L2, 210 MB of them hits, 30 GB/s for each compute unit) and 55 us at rank 16
+// (MS = 1: more wavefronts; MS = 2 takes 61).  16 column blocks a unit: 32 take 56 and 62 us.
 template <int DT, int MS, int KQ, int PMAX>  // ranks up to 64 * KQ and, below 64, up to 8 * PMAX
 __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_expand_kernel(AdapterArgs g) {
   // [4][64 * P] pieces of B, then [2][16*MS][kp + 8]: hi and lo of v, kp = r rounded up to 32 (16)
@@ -579,8 +582,9 @@ __global__ __launch_bounds__(256, MS == 2 ? 3 : PMAX == 4 ? 5 : 4) void adapter_
 // Eight wavefronts, 16 sorted rows of one adapter and a unit of columns of one slice.  The first product is made anew by
 // every block of a row block (its operands come from the L2), which saves the launch between the two and the way of v
 // through memory.  The blocks of a row block have numbers 8 apart: they run on one XCD and share its L2.
-// Bound by latency: the launch and a chain of four trips to memory.  One token, rank 16, 7168 -> 2 x 2048: 8.5 us.  64 tokens
-// with 64 adapters, rank 16, 2048 -> 7168: 11.1 us for 21 MB.
+// Bound by latency: the launch and, at H = 7168 and rank 16, six trips to memory in a row (offsets, tokens, and a wavefront's 14
+// chunks four at a time).  One token, rank 16, 7168 -> 2 x 2048: 8.5 us.  64 tokens, each with an adapter of its own (some 56 of 64; the
+// others have none), rank 16, 2048 -> 7168: 11 us for 19 MB.
 constexpr int FUSED_WAVES = 8;
 template <int DT, int RT>
 __global__ __launch_bounds__(FUSED_WAVES * WAVE) void adapter_fused_kernel(AdapterArgs g) {

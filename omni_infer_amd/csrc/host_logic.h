@@ -573,10 +573,12 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
   AdapterPlan p{};
   const int R = r * n_slices, cols = (N + 63) / 64;
   // One launch: 16 rows a block.  Its blocks make the first product anew, each reads a slice of A, as often as there are
-  // units of columns.  Measured on the GPU: 8.5 us against 7.7 us in two launches for one token (rank 16, 7168 -> 2 x 2048),
-  // 11.2 against 14.2 us for 64 tokens with 64 adapters (rank 16, 2048 -> 7168), 8.3 against 9.9 us for 333 tokens with 12
-  // (rank 24, 1992 -> 1048); called from Python, where a launch costs the host 3 us and the workspace another, 11.5 against
-  // 16.5 us.  A slice of 256 KB and 64 MB over all blocks are where one launch stops paying.
+  // units of columns.  The limits (a slice of 256 KB, 64 MB over all blocks, 1024 tokens) were set from calls out of Python,
+  // where a second launch costs the host 3 us and the workspace another (one token, rank 16, 7168 -> 2 x 2048: 11.5 against
+  // 16.5 us).  Replayed from a graph, one launch against two: rank 16, 2048 -> 7168: 1 token 5.7 / 7.3 us, 64 of 64 adapters
+  // 12.3 / 12.9, 512 of 8 11.7 / 13.3; rank 16, 7168 -> 2 x 2048: 1 token 8.6 / 8.0, 64 of 64 13.8 / 15.5, 512 of 8 13.7 / 14.5,
+  // but 1000 of 8 27.5 / 18.1; outside the limits rank 32: 1 token 10.0 / 9.0, 64 of 64 16.7 / 19.8 (the rule loses that
+  // one), 1000 of 8 32.7 / 20.8; rank 64: 1 token 16.4 / 11.6, 512 of 8 21.9 / 21.7.
   if (r <= 64 && (int64_t)r * H * 2 <= 256 << 10) {
     const int64_t tiles = T / 16 + imin(n, T) + 1;
     const int64_t want = 256 / tiles;  // units of columns for a block on every compute unit
@@ -591,17 +593,32 @@ inline AdapterPlan adapter_plan(int T, int n, int H, int r, int n_slices, int N)
       return p;
     }
   }
+  // The tile kernel from 1024 tokens on, 32 to an adapter: both products of 7168 -> 2 x 2048 with it / with 16-row blocks, in
+  // graph replay: rank 64: 512 tokens of 4 24.2 / 23.0 us, 1024 28.4 / 27.0, 2048 37.7 / 37.8, 4096 63.3 / 73.0, 8192
+  // 91.4 / 143; rank 16: 8192 62.8 / 79.7; under 32 rows an adapter: 2048 tokens of 128, rank 64 96.1 / 85.9.  Where x is narrow
+  // and the rank low it gains nothing (rank 16, 2048 -> 7168: 1024 tokens 20.3 / 16.9, 8192 68.4 / 67.5), and at 32 rows an
+  // adapter it still loses with rank 16 (8192 tokens of 256: 144 / 106; rank 64: 222 / 220).
   const bool many = T >= 1024 && T / 32 >= n;
   p.rank_block = R <= 16 && !many ? 16 : R <= 32 && !many ? 32 : R <= 64 ? 64 : 128;
   p.row_tiles = many ? 8 : 1;
   p.tiles_max = T / (16 * p.row_tiles) + imin(n, T);
   const int chunks = (H + 63) / 64;
   const int64_t blocks = (int64_t)p.tiles_max * ((R + p.rank_block - 1) / p.rank_block);
-  int64_t k = 512 / blocks;  // two blocks per compute unit
+  // Two blocks per compute unit: at 8192 tokens, rank 64, 7168 -> 2 x 2048 91 us, one block 102, four 105 (512 tokens: 21.5,
+  // 20.4, 23.1).  Eight chunks a part at least: one token, rank 64 11.5 us, with four 11.6, with sixteen 12.7 (1024 tokens: 28.2,
+  // 27.8, 31.2).  16 parts at most: one token, rank 64, 16384 -> 7168 12.1 us, with 8 13.9, with 32 12.3; 1100 tokens,
+  // 16384 -> 1024 25.4, 31.5, 27.9.
+  int64_t k = 512 / blocks;
   if (k > chunks / 8) k = chunks / 8;
   p.ksplit = k < 1 ? 1 : k > 16 ? 16 : (int)k;
-  p.out_row_tiles = many && r > 32 && r <= 128 ? 2 : 1;  // what the second product keeps in LDS stays below 64 KB
+  // Two row tiles halve the reads of B and of the parts: 8192 tokens, 7168 -> 2 x 2048, both products with two / one: rank 40
+  // 85.0 / 86.1 us, 64 91.3 / 94.6, 96 118.4 / 126.0, 128 121.7 / 130.6; not at rank 16 67.7 / 62.1 and 32 73.3 / 70.6 (fewer
+  // wavefronts).  Past 128 what the second product keeps in LDS would exceed 64 KB.
+  p.out_row_tiles = many && r > 32 && r <= 128 ? 2 : 1;
   p.out_tiles_max = T / (16 * p.out_row_tiles) + imin(n, T);
+  // 4 column blocks a unit / 16: one token, rank 64 11.5 / 15.2 us, 512 tokens of 8 21.6 / 24.1; 8192 tokens 101.7 / 91.4 and, rank
+  // 16, 2048 -> 7168, 94.7 / 70.1.  In between it is about even (64 tokens of 64 26.8 / 29.0, 2048 tokens 39.1 / 37.3; with 8
+  // 27.1 and 34.4).
   p.unit_blocks = p.out_tiles_max > 64 ? 16 : 4;
   return p;
 }

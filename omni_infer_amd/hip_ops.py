@@ -495,6 +495,8 @@ def _join_plan(plan: AdapterPlan, device: int) -> None:
     memory, so neither a sort that has not run yet nor memory that was given to someone else may be read.  A stream being
     captured cannot wait for work outside; the capture's own start lies behind the plan."""
     raw = torch._C._cuda_getCurrentRawStream(device)
+    if plan.stream is None and not _capturing(device):
+        raise RuntimeError("adapter_linear: the plan was made inside a graph capture and holds nothing outside of it")
     if raw in plan.joined:
         return
     stream = torch.cuda.current_stream(device)
@@ -511,7 +513,8 @@ def adapter_plan(adapter_ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
     token; a value outside [0, n_adapters) (-1, say) means none.  Made once for a batch and used by all its
     projections, also on other streams: the first use there waits for what the plan's stream has been given so far.  A
     graph that uses a plan made outside of it reads the plan's memory at every replay, so the plan has to live as long
-    as the graph; one made inside is made anew by every replay and means nothing before the first."""
+    as the graph; one made inside is made anew by every replay and refused outside of a capture: before the first replay
+    it would name places anywhere."""
     device = _one_device("adapter_plan", adapter_ids)
     if adapter_ids.dim() != 1 or adapter_ids.dtype not in (torch.int32, torch.int64):
         raise ValueError("adapter_plan: adapter_ids must be [T], int32 or int64")

@@ -94,8 +94,15 @@ def test_a_plan_joins_the_stream_that_uses_it(capturing, monkeypatch):
     assert buf.log == (want * 2 if capturing else want)      # once for a stream
     plan.stream, plan.joined = None, {7}                       # made inside a capture: its streams are joined by whoever captures
     del buf.log[:]
-    ops._join_plan(plan, 0)
-    assert buf.log == [("record", 9)]
+    if capturing:
+        ops._join_plan(plan, 0)
+        assert buf.log == [("record", 9)]
+        return
+    for raw in (7, 9):                                        # before a replay its places could be anywhere
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: raw, raising=False)
+        with pytest.raises(RuntimeError, match="capture"):
+            ops._join_plan(plan, 0)
+    assert buf.log == []
 
 
 @pytest.mark.gpu
@@ -279,3 +286,33 @@ def test_two_graphs_with_workspaces():
         torch.cuda.synchronize()
         for d, _, got in made:
             assert torch.equal(got, run(d)), k
+
+
+@pytest.mark.gpu
+def test_a_plan_of_a_capture_stays_in_captures():
+    """Refused outside, on the capture's own stream too; used on a second stream that the capture forks to and joins."""
+    from omni_infer_amd import hip_ops as ops
+    T, n, r, H, widths = FORMS[2]
+    d = make(T, n, r, H, widths, BF16, seed=2)
+    want = run(d)
+    call = lambda plan: ops.adapter_linear(d["x"], d["base"], d["a"], d["b"], plan, d["scale"], slices=d["widths"])  # noqa: E731
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main):
+        plan = ops.adapter_plan(d["ids"], n)
+        here = call(plan)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            there = call(plan)
+        main.wait_stream(side)
+    for s in (torch.cuda.current_stream(), main, side):
+        with torch.cuda.stream(s), pytest.raises(RuntimeError, match="capture"):
+            call(plan)
+    for k in range(3):
+        d["ids"].copy_(torch.randint(-1, n, (T,), dtype=torch.int32, generator=torch.Generator().manual_seed(k)))
+        want = run(d)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(here, want) and torch.equal(there, want)
